@@ -119,3 +119,7 @@ def gemm_bf16_tn(a, b, out=None, trans_out=False, dual_off=0, splitk=0, bn=0, ou
         out = torch.empty(shape, device=a.device, dtype=out_dtype or torch.bfloat16)
     _C.gemm_bf16_tn(a, b, out, trans_out, dual_off, splitk, bn, a_tiled_rows)
     return out
+
+
+from .kv_cache import (KVBlocks, KVCache8, KVPlan, decode_attention_8bit, kv_append_8bit, kv_plan, kv_release)  # noqa: E402,F401
+from .logprobs import TokenLogprobs, token_logprobs  # noqa: E402,F401
