@@ -268,7 +268,7 @@ void attention(const Tensor& qkv, const Tensor& positions, const Tensor& table, 
   p.table_rows = (int)cos.size(0);
   p.scale = 1.0f / std::sqrt((float)k.size(3));
   p.cache = cache_of(k, v, ks, vs, kt, vt);
-  p.nsplit = ccl::decode_attention8_splits(p);
+  ccl::decode_attention8_split(p);
   p.partials = nullptr;
   Tensor partials;  // of this call alone: two calls, or two captured graphs, never share it
   if (const size_t n = ccl::decode_attention8_partial_floats(p)) {

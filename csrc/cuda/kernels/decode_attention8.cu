@@ -9,11 +9,14 @@
 // and no barrier in the loop. (tcgen05 wants its operands in shared memory, widened: a round trip for every byte and 128 rows for at most
 // 16; with eight rows the products take a sixth of the time that the bytes take to arrive.)
 //
-// Exactness. Codes widen to f16 without rounding. q is multiplied by a power of two that brings its largest element to 2^9 .. 2^10 and
-// split into two f16 parts (22 bits), so scores are as exact as in fp32. The page's V scale joins the score, as log2(scale): weights
-// 2^(s + log2 vs - m) multiply the codes in f16, kept within a factor of 2^15 of the running reference, and the sum of the softmax takes
-// them divided by vs, in fp32. The reference m moves only when a score passes it by 2^15, and starts 2^8 below the maximum.
-// The tail (bf16, at most a block) is done in fp32 on the CUDA cores.
+// Exactness. Codes widen to f16 without rounding. q is multiplied by a power of two and split into two f16 parts (22 bits), so scores are
+// as exact as in fp32. The page's V scale joins the score, as log2(scale): weights 2^(s + log2 vs - m) multiply the codes in f16, kept
+// within a factor of 2^15 of the running reference, and the sum of the softmax takes them divided by vs, in fp32. The reference m moves
+// only when a score passes it by 2^15, and starts 2^8 below the maximum. The tail (bf16, at most a block) goes through the same products in
+// bf16, q in three parts and the weights in two.
+//
+// A warp takes two units of 16 positions at a time, so that a fragment of q is read once for both, and has the next two pairs on their way:
+// every thread copies (cp.async) what it will read itself, which needs no barrier. 64 KB of ring let three CTAs of four warps share an SM.
 #include "kv_cache8.cuh"
 
 #include "gemm.h"
@@ -27,20 +30,23 @@ using namespace kv8;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMinUnits = 16;      // units of 16 positions per split at least: four for each warp
+constexpr int kStages = 2;         // pairs of units on their way to a warp, or in use
+constexpr int kMaxSplits = 64, kMaxCluster = 16;
+constexpr int kLeast = 8;          // units of 16 positions per split at least: a pair for each warp
+constexpr int kChunk = 512;        // units of a split where there are CTAs enough without splits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHead = 8.f;       // the reference starts this far (log2) below the maximum
 constexpr float kRoom = 15.f;      // and moves when a weight would pass 2^15 (f16 ends at 2^16)
 
-// Work split of one sequence: `per` units of 16 paged positions for each of `used` splits; the last one takes the tail too.
+// Work split of one sequence and head tile: `per` units of 16 paged positions for each of `used` splits; the last one takes the tail too.
 struct Split {
   int units, per, used;
 };
-__device__ __forceinline__ Split split_of(int pos, int block, int nsplit) {
+__device__ __forceinline__ Split split_of(int pos, const DecodeAttn8Params& p) {
   Split s;
-  s.units = (pos / block) * (block / 16);
-  s.per = max(kMinUnits, (s.units + nsplit - 1) / nsplit);
-  s.used = max(1, (s.units + s.per - 1) / s.per);
+  s.units = (pos / p.cache.block) * (p.cache.block / 16);
+  s.per = max(p.least, (s.units + p.nsplit - 1) / p.nsplit);
+  s.used = max(1, (s.units + s.per - 1) / s.per);  // at most nsplit
   return s;
 }
 __device__ __forceinline__ bool position_ok(const DecodeAttn8Params& p, int pos) {
@@ -48,15 +54,20 @@ __device__ __forceinline__ bool position_ok(const DecodeAttn8Params& p, int pos)
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
+}
+__device__ __forceinline__ float2 ld_cluster(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -67,65 +78,180 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Four codes -> two f16 pairs, exactly.
-template <bool INT8>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (INT8) {
-    w ^= 0x80808080u;  // 0 .. 255 in the mantissa of 1024 + u, then minus 1152
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));
-    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias), y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-  }
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 or 8 bytes to shared memory, or zeros (`bytes` 0).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Four e4m3 codes -> two f16 pairs, exactly. The conversion instruction runs on a unit that starts 16 lanes a clock on a multiprocessor; for
+// all of K and V it would bound the loop, so half of K goes the other way:
+__device__ __forceinline__ void widen_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// ... 2^-8 of their values, on the integer units: a code's seven lower bits, moved to bit 7, are the f16 whose exponent is read with a bias
+// that is 8 larger, denormals too. (The NaN code has a NaN scale.)
+constexpr float kLowE4m3 = 256.f;
+__device__ __forceinline__ void widen_e4m3_low(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t x = __byte_perm(w, 0, 0x1100), y = __byte_perm(w, 0, 0x3322);
+  lo = ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
+  hi = ((y >> 1) & 0x3f803f80u) | (y & 0x80008000u);
+}
+// Four int8 codes -> (code + 128) * 2^-24 as denormal f16: K's products then have 128 * sum(q) too much, which is taken off the scores.
+constexpr float kLowInt8 = 16777216.f;
+__device__ __forceinline__ void widen_int8_low(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  lo = __byte_perm(w, 0, 0x4140);
+  hi = __byte_perm(w, 0, 0x4342);
+}
+// Four int8 codes plus 128 -> the codes: 1024 + u as f16, minus 1152. (V's weights are not known beforehand, and its sums cancel: no bias.)
+__device__ __forceinline__ void widen_biased(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias), y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
 }
 
 template <int D, int NT>
 struct Smem {
   static constexpr int R = 8 * NT;       // query rows
   static constexpr int QP = D + 4;       // pitch (halves): eight rows start two banks apart
-  static constexpr int OP = D + 4;       // pitch (floats)
-  __half qh[R * QP], ql[R * QP];         // q as two f16 parts
-  float qf[R * D];                       // q in fp32, for the tail
-  float o[kWarps][R * OP];               // out of each warp
-  float m[kWarps][R], l[kWarps][R];
+  static constexpr int OS = D / 8 + 2;   // the dims of a lane (floats), moved two banks on for each g
+  static constexpr int OP = 8 * OS + 2;  // pitch (floats)
+  static constexpr int kUnit = 16 * D;   // bytes of K, or of V, of a unit of 16 positions
+  union {
+    uint8_t ring[kWarps][kStages][2][2 * kUnit];  // K and V of two units
+    struct {                             // at the end
+      float o[kWarps][R * OP];           // out of each warp
+      float2 joined[R * (D / 2 + 1)];    // of the CTA, for the others of its cluster: out, and {m, l} behind each row
+    };
+  };
+  union {
+    struct {
+      __half qh[R * QP], ql[R * QP];     // q as two f16 parts
+    };
+    struct {
+      float m[kWarps][R], l[kWarps][R];  // at the end
+    };
+  };
+  __nv_bfloat16 qb[3][R * QP];           // q as three bf16 parts, for the tail
   float qs[R];                           // scale * log2 e over the power of two of the row
-  uint32_t new_k[D / 2], new_v[D / 2];   // the new token, bf16
+  float qc[R];                           // int8: what the codes' bias adds to a score
+  uint4 new_k[D / 8], new_v[D / 8];      // the new token, bf16
   uint32_t amax[2][kWarps];
   int bad;
 };
 
-// Quantises the block that the new token completes. `src`: 0 for K, 1 for V.
+// The new token of one sequence and KV head: k rotated, both as bf16 in shared memory. Two words (four values) a thread, of D / 2 threads;
+// `load` needs no position.
+struct NewToken {
+  uint32_t a, b;
+};
+template <int D>
+__device__ __forceinline__ NewToken load_new(const DecodeAttn8Params& p, int b, int kvh) {
+  const int tid = threadIdx.x, i = tid & (D / 4 - 1);
+  if (tid >= D / 2) return {0, 0};
+  const int head = p.n_heads + kvh + (tid < D / 4 ? 0 : p.cache.n_kv_heads);  // the first D / 4 threads have k, the others v
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(p.qkv + (size_t)b * p.qkv_stride + (size_t)head * D) + i;
+  return {src[0], src[D / 4]};
+}
+template <int D>
+__device__ __forceinline__ void store_new(const DecodeAttn8Params& p, NewToken w, int pos, uint4* k, uint4* v) {
+  static_assert(kThreads >= D / 2, "a thread for each pair of words of k, and of v");
+  const int tid = threadIdx.x, i = tid & (D / 4 - 1);
+  if (tid >= D / 2) return;
+  if (tid < D / 4) {  // dims 2i and 2i + 1 and the ones half a head further on
+    const float2 c = reinterpret_cast<const float2*>(p.cos + (size_t)pos * (D / 2))[i], s = reinterpret_cast<const float2*>(p.sin + (size_t)pos * (D / 2))[i];
+    float x0, y0, x1, y1;
+    rotate(lo_f(w.a), lo_f(w.b), c.x, s.x, x0, y0);
+    rotate(hi_f(w.a), hi_f(w.b), c.y, s.y, x1, y1);
+    w.a = pack_bf16(x0, x1);
+    w.b = pack_bf16(y0, y1);
+  }
+  uint32_t* dst = reinterpret_cast<uint32_t*>(tid < D / 4 ? k : v) + i;
+  dst[0] = w.a;
+  dst[D / 4] = w.b;
+}
+
+// Quantises the block that the new token completes. A CTA of its own does that, beside the attention (which reads this block from the
+// tail): within the CTA that attends it took as long as 300 positions.
 template <int D, bool INT8>
-__device__ __forceinline__ void quantise_block(const __nv_bfloat16* tail, const uint32_t* fresh, int block, uint32_t (&amax)[kWarps], uint8_t* page, float* scale_out) {
-  const int tid = threadIdx.x, n = block * D / 4;  // pieces of four values
-  const int last = (block - 1) * (D / 4);          // from here on: the new token
-  auto piece = [&](int i) {
-    return i >= last ? make_uint2(fresh[(i - last) * 2], fresh[(i - last) * 2 + 1]) : *reinterpret_cast<const uint2*>(tail + (size_t)i * 4);
-  };
-  uint32_t seen = 0;
-  for (int i = tid; i < n; i += kThreads) {
-    const uint2 w = piece(i);
-    seen = amax_bits(amax_bits(seen, w.x), w.y);
-  }
-  seen = __reduce_max_sync(0xffffffffu, seen);
-  if ((tid & 31) == 0) amax[tid >> 5] = seen;
+__device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b, int kvh, uint4* fresh_k, uint4* fresh_v, uint32_t (*amax)[kWarps]) {
+  const KvCache8& c = p.cache;
+  const int tid = threadIdx.x, pos = p.positions[b];
+  if (!position_ok(p, pos) || (pos & (c.block - 1)) != c.block - 1) return;
+  const int page = p.table[(size_t)b * p.max_blocks + pos / c.block];
+  if ((unsigned)page >= (unsigned)c.num_blocks) return;
+  store_new<D>(p, load_new<D>(p, b, kvh), pos, fresh_k, fresh_v);
   __syncthreads();
-  seen = 0;
+  const size_t at = ((size_t)b * c.n_kv_heads + kvh) * c.block * D, sc = (size_t)page * c.n_kv_heads + kvh;
+  const uint4* k = reinterpret_cast<const uint4*>(c.k_tail + at);
+  const uint4* v = reinterpret_cast<const uint4*>(c.v_tail + at);
+  const int last = (c.block - 1) * (D / 8), n = last + D / 8;  // pieces of eight values; from `last` on: the new token
+  constexpr int U = 8;                                          // of K, and of V, in flight
+  uint4 x[U], y[U];
+  auto fetch = [&](int i0) {
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) seen = max(seen, amax[w]);
-  const float scale = scale_of<INT8>(bits_f(seen));
-  for (int i = tid; i < n; i += kThreads) {
-    const uint2 w = piece(i);
-    *reinterpret_cast<uint32_t*>(page + (size_t)i * 4) = codes4<INT8>(lo_f(w.x), hi_f(w.x), lo_f(w.y), hi_f(w.y), scale);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      x[u] = y[u] = make_uint4(0, 0, 0, 0);
+      if (i < n) {
+        x[u] = *(i >= last ? fresh_k + (i - last) : k + i);
+        y[u] = *(i >= last ? fresh_v + (i - last) : v + i);
+      }
+    }
+  };
+  auto most = [](uint32_t seen, const uint4& w) { return amax_bits(amax_bits(amax_bits(amax_bits(seen, w.x), w.y), w.z), w.w); };
+  uint32_t seen_k = 0, seen_v = 0;
+  for (int i0 = tid; i0 < n; i0 += U * kThreads) {
+    fetch(i0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) seen_k = most(seen_k, x[u]), seen_v = most(seen_v, y[u]);
   }
-  if (tid == 0) *scale_out = scale;
+  seen_k = __reduce_max_sync(0xffffffffu, seen_k);
+  seen_v = __reduce_max_sync(0xffffffffu, seen_v);
+  if ((tid & 31) == 0) amax[0][tid >> 5] = seen_k, amax[1][tid >> 5] = seen_v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) seen_k = max(seen_k, amax[0][w]), seen_v = max(seen_v, amax[1][w]);
+  const float scale_k = scale_of<INT8>(bits_f(seen_k)), scale_v = scale_of<INT8>(bits_f(seen_v));
+  uint2* to_k = reinterpret_cast<uint2*>(c.k + sc * c.block * D);
+  uint2* to_v = reinterpret_cast<uint2*>(c.v + sc * c.block * D);
+  auto codes8 = [](const uint4& w, float scale) {
+    return make_uint2(codes4<INT8>(lo_f(w.x), hi_f(w.x), lo_f(w.y), hi_f(w.y), scale), codes4<INT8>(lo_f(w.z), hi_f(w.z), lo_f(w.w), hi_f(w.w), scale));
+  };
+  for (int i0 = tid; i0 < n; i0 += U * kThreads) {
+    if (n > U * kThreads) fetch(i0);  // (a block of one round is still there)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i < n) {
+        to_k[i] = codes8(x[u], scale_k);
+        to_v[i] = codes8(y[u], scale_v);
+      }
+    }
+  }
+  if (tid == 0) {
+    c.k_scale[sc] = scale_k;
+    c.v_scale[sc] = scale_v;
+  }
 }
 
 template <int D, int NT, bool INT8>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) decode_attention8_kernel(const DecodeAttn8Params p) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_kernel(const DecodeAttn8Params p) {
   constexpr int R = 8 * NT;
   constexpr int KJ = D / 64;        // 16-byte loads of a K row by a thread
   constexpr int VW = D / 32;        // words of a V row by a thread
@@ -141,148 +267,196 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) decode_attention8_k
   const int g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / c.n_kv_heads;
   const int tiles = (group + R - 1) / R;
-  const int kvh = blockIdx.y / tiles, tile = blockIdx.y - kvh * tiles;
+  // the grid: nsplit CTAs for every pair of a head tile and a sequence; then, the last to start, one for each sequence and KV head whose
+  // block may fill up
+  const int pairs = p.batch * c.n_kv_heads * tiles;
+  const int pair = blockIdx.x / p.nsplit, split = blockIdx.x - pair * p.nsplit;
+  if (pair >= pairs) {
+    const int i = (pair - pairs) * p.nsplit + split;
+    if (i < p.batch * c.n_kv_heads) quantise_block<D, INT8>(p, i % p.batch, i / p.batch, sm.new_k, sm.new_v, sm.amax);
+    return;
+  }
+  const int b = pair % p.batch, kvh = pair / p.batch / tiles, tile = pair / p.batch - kvh * tiles;
   const int rows = min(R, group - tile * R);
   const int head0 = kvh * group + tile * R;
-  const int b = blockIdx.z, split = blockIdx.x;
   const int pos = p.positions[b];
+  // what needs no position is asked for with it: q (LPR lanes share a row; a lane has two words of it, half a head apart), the new token
+  constexpr int LPR = D / 4, RPW = 32 / LPR, QI = R / (kWarps * RPW);
+  const int q_word = lane % LPR;
+  uint32_t q_lo[QI], q_hi[QI];
+  auto q_row = [&](int i) { return (i * kWarps + warp) * RPW + lane / LPR; };
+#pragma unroll
+  for (int i = 0; i < QI; ++i) {
+    q_lo[i] = q_hi[i] = 0;
+    if (q_row(i) < rows) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.qkv + (size_t)b * p.qkv_stride + (size_t)(head0 + q_row(i)) * D) + q_word;
+      q_lo[i] = src[0];
+      q_hi[i] = src[D / 4];
+    }
+  }
+  const NewToken fresh = load_new<D>(p, b, kvh);
   __nv_bfloat16* out = p.out + (size_t)b * p.out_stride + (size_t)head0 * D;
   if (!position_ok(p, pos)) {
     if (split == 0)
       for (int i = tid; i < rows * D; i += kThreads) out[i] = __float2bfloat16(0.f);
     return;
   }
-  const Split sp = split_of(pos, c.block, p.nsplit);
+  const Split sp = split_of(pos, p);
   if (split >= sp.used) return;
   const bool owns_tail = split == sp.used - 1;
   const int* table = p.table + (size_t)b * p.max_blocks;
 
-  // ---- the loop's loads: unit n of this warp is unit u0 + warp + 4 n of the sequence -------------------------------------------
-  const int u0 = split * sp.per, u1 = min(sp.units, u0 + sp.per);
-  const int n_units = max(0, (u1 - u0 - warp + kWarps - 1) / kWarps);
+  // ---- the loop's loads: units of the split in pairs, pair n of this warp being pair warp + 4 n -----------------------------------
+  const int u0 = split * sp.per, units = max(0, min(sp.units - u0, sp.per));
+  const int n_pairs = max(0, ((units + 1) / 2 - warp + kWarps - 1) / kWarps);
   const int in_block = 31 - __clz(c.block / 16);  // log2 of the units of a block
+  const int place = pos & (c.block - 1);
+  // the tail's units of 16 positions follow the pairs, the first of them with the last warp
+  const int tail_units = owns_tail ? place / 16 + 1 : 0;
+  const int n_all = n_pairs + max(0, (tail_units - (kWarps - 1 - warp) + kWarps - 1) / kWarps);
+  auto tail_first = [&](int n) { return ((kWarps - 1 - warp) + kWarps * (n - n_pairs)) * 16; };
+  const size_t tail_at = ((size_t)b * c.n_kv_heads + kvh) * c.block * D;
   bool bad = false;
-  auto page_of = [&](int n) {  // of the window's lane
-    int page = 0;
-    if (n < n_units) {
-      page = table[(u0 + warp + kWarps * n) >> in_block];
-      if ((unsigned)page >= (unsigned)c.num_blocks) {
-        bad = true;
-        page = 0;
-      }
-    }
-    return page;
+  // a window of 16 pairs: each lane looks up the page of one unit, and its scales
+  auto unit_of = [&](int n, int h) { return 2 * (warp + kWarps * n) + h; };
+  auto page_of = [&](int n) {  // of window n / 16, for this lane
+    const int u = unit_of(n + (lane >> 1), lane & 1);
+    if (u >= units) return 0;
+    const int page = table[(u0 + u) >> in_block];
+    if ((unsigned)page < (unsigned)c.num_blocks) return page;
+    bad = true;
+    return 0;
   };
-  // a window of 32 units: each lane looks up one page and its scales
-  int pages = page_of(lane), pages_next = page_of(32 + lane);
+  int pages = page_of(0), pages_next = page_of(16);
   float ks_next = 1.f, vs_next = 1.f;
   auto scales_of = [&](int n) {
-    if (n < n_units) {
-      const size_t at = (size_t)pages * c.n_kv_heads + kvh;
-      ks_next = c.k_scale[at];
-      vs_next = c.v_scale[at];
-    }
+    if (unit_of(n + (lane >> 1), lane & 1) >= units) return;
+    const size_t at = (size_t)pages * c.n_kv_heads + kvh;
+    ks_next = c.k_scale[at];
+    vs_next = c.v_scale[at];
   };
-  uint4 kr[2][KJ];
-  uint32_t vr[4][VW];
-  size_t at = 0;  // byte offset of the unit in both pools
-  auto load_k = [&](int n) {
-    if (n >= n_units) return;  // uniform
-    if (n > 0 && (n & 31) == 0) {
-      pages = pages_next;
-      scales_of(n + lane);
-      pages_next = page_of(n + 32 + lane);
-    }
-    const int page = __shfl_sync(0xffffffffu, pages, n & 31);
-    const int u = u0 + warp + kWarps * n;
-    at = (((size_t)page * c.n_kv_heads + kvh) * c.block + (size_t)(u & ((1 << in_block) - 1)) * 16) * D;
-    const uint8_t* k = c.k + at + g * D + t * 16;
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) {
-      kr[0][j] = ptx::ld_nc_v4(k + j * 64);
-      kr[1][j] = ptx::ld_nc_v4(k + 8 * D + j * 64);
-    }
-  };
-  auto load_v = [&](int n) {
-    if (n >= n_units) return;
-    const uint8_t* v = c.v + at + g * (D / 8);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* row = v + (2 * t + (i & 1) + (i >> 1) * 8) * D;
-      if constexpr (VW == 4) {
-        const uint4 x = ptx::ld_nc_v4(row);
-        vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
-      } else {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row));
-        vr[i][0] = x.x, vr[i][1] = x.y;
+  // A thread copies what it will read itself: K's rows g and g + 8, V's rows 2t, 2t + 1, 2t + 8, 2t + 9.
+  const uint32_t page_bytes = (uint32_t)c.n_kv_heads * c.block * D;  // at most 2^30
+  const uint8_t* k_base = c.k + (size_t)kvh * c.block * D + g * D + t * 16;
+  const uint8_t* v_base = c.v + (size_t)kvh * c.block * D + 2 * t * D + g * (D / 8);
+  const uint32_t ring = ptx::smem_u32(sm.ring[warp]);
+  // A row of V that a load brings in stays together in shared memory (scattered by thread, its 16 bytes would be written one after the
+  // other: 5.2 instead of 7.0 TB/s); its pieces change places with the row, so that they are read without conflicts.
+  const uint32_t v_place = t * D + (D == 128 ? (g ^ (2 * t)) * 16 : (g ^ (2 * (t & 2))) * 8);
+  size_t at[kStages][2];
+  auto load_k = [&](int n, size_t (&where)[2]) {
+    if (n < n_pairs) {
+      if (n > 0 && (n & 15) == 0) {
+        pages = pages_next;
+        scales_of(n);
+        pages_next = page_of(n + 16);
       }
-    }
-  };
-  scales_of(lane);
-  load_k(0);
-  load_v(0);
-
-  // ---- q: rotate, split; the new token ------------------------------------------------------------------------------------------
-  const __nv_bfloat16* qkv = p.qkv + (size_t)b * p.qkv_stride;
-  const float* cosr = p.cos + (size_t)pos * (D / 2);
-  const float* sinr = p.sin + (size_t)pos * (D / 2);
-  constexpr int PP = D / 64;  // rotated pairs of a lane
-  for (int r = warp; r < R; r += kWarps) {
-    float x[PP], y[PP], most = 0.f;
-#pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const int d = lane + 32 * i;
-      x[i] = y[i] = 0.f;
-      if (r < rows) {
-        const __nv_bfloat16* src = qkv + (size_t)(head0 + r) * D;
-        rotate(__bfloat162float(src[d]), __bfloat162float(src[d + D / 2]), cosr[d], sinr[d], x[i], y[i]);
-      }
-      most = fmaxf(most, fmaxf(fabsf(x[i]), fabsf(y[i])));
-    }
-    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-    const int e = (int)(__float_as_uint(most) >> 23);  // biased exponent; 0 for a row of zeros, 255 for an infinity
-    const int up = e == 0 || e == 255 ? 127 : min(254, 127 + 9 + 127 - e);
-    const float mult = __uint_as_float((uint32_t)up << 23);
-#pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const int d = lane + 32 * i;
-      const float z[2] = {x[i], y[i]};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int dd = d + h * (D / 2);
-        const float v = z[h] * mult;
-        const __half hi = __float2half_rn(v);
-        sm.qh[r * S::QP + dd] = hi;
-        sm.ql[r * S::QP + dd] = __float2half_rn(v - __half2float(hi));
-        sm.qf[r * D + dd] = z[h];
+        const int u = unit_of(n, h);
+        const uint32_t page = __shfl_sync(0xffffffffu, pages, 2 * (n & 15) + h);
+        where[h] = (size_t)page * page_bytes + (uint32_t)(((u0 + u) & ((1 << in_block) - 1)) * 16 * D);
+        const uint8_t* k = k_base + where[h];
+        const uint32_t dst = ring + ((n % kStages) * 2 * 2 + h) * S::kUnit + lane * 16, bytes = u < units ? 16 : 0;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          copy16(dst + j * 1024, k + j * 64, bytes);
+          copy16(dst + j * 1024 + 512, k + 8 * D + j * 64, bytes);
+        }
+      }
+    } else if (n < n_all) {  // bf16: one unit is as long as two of codes; the new position is not in the tail yet
+      const int r = tail_first(n) + g;
+      const __nv_bfloat16* k = c.k_tail + tail_at + (size_t)g * D + (size_t)tail_first(n) * D + t * 8;
+      const uint32_t dst = ring + (n % kStages) * 4 * S::kUnit + lane * 16, b0 = r < place ? 16 : 0, b8 = r + 8 < place ? 16 : 0;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        copy16(dst + j * 1024, r < place ? k + j * 32 : c.k_tail, b0);
+        copy16(dst + j * 1024 + 512, r + 8 < place ? k + 8 * D + j * 32 : c.k_tail, b8);
       }
     }
-    if (lane == 0) sm.qs[r] = p.scale * kLog2e / mult;
+    copies_done();
+  };
+  auto load_v = [&](int n, const size_t (&where)[2]) {
+    if (n < n_pairs) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* v = v_base + where[h];
+        const uint32_t dst = ring + ((n % kStages) * 2 * 2 + 2 + h) * S::kUnit + v_place, bytes = unit_of(n, h) < units ? D / 8 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* row = v + ((i & 1) + (i >> 1) * 8) * D;
+          if constexpr (D == 128)
+            copy16(dst + i * 512, row, bytes);
+          else
+            copy8(dst + i * 256, row, bytes);
+        }
+      }
+    } else if (n < n_all) {
+      const uint32_t dst = ring + ((n % kStages) * 4 + 2) * S::kUnit + lane * 16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = tail_first(n) + 2 * t + (i & 1) + (i >> 1) * 8;
+        const __nv_bfloat16* v = r < place ? c.v_tail + tail_at + (size_t)r * D + g * (D / 8) : c.v_tail;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) copy16(dst + (i * (D / 64) + j) * 512, v + j * 8, r < place ? 16 : 0);
+      }
+    }
+    copies_done();
+  };
+  scales_of(0);
+#pragma unroll
+  for (int n = 0; n < kStages; ++n) {
+    load_k(n, at[n]);
+    load_v(n, at[n]);
   }
-  const int place = pos & (c.block - 1);
-  const size_t tail_at = ((size_t)b * c.n_kv_heads + kvh) * c.block * D;
-  if (owns_tail && tid < D / 2) {
-    // thread i < D/4 holds dims 2i, 2i + 1 of K and their partners; the others V
-    const __nv_bfloat16* kn = qkv + (size_t)(p.n_heads + kvh) * D;
-    const __nv_bfloat16* vn = kn + (size_t)c.n_kv_heads * D;
-    if (tid < D / 4) {
-      const uint32_t a = reinterpret_cast<const uint32_t*>(kn)[tid], h = reinterpret_cast<const uint32_t*>(kn)[tid + D / 4];
-      float x0, y0, x1, y1;
-      rotate(lo_f(a), lo_f(h), cosr[2 * tid], sinr[2 * tid], x0, y0);
-      rotate(hi_f(a), hi_f(h), cosr[2 * tid + 1], sinr[2 * tid + 1], x1, y1);
-      sm.new_k[tid] = pack_bf16(x0, x1);
-      sm.new_k[tid + D / 4] = pack_bf16(y0, y1);
-    } else {
-      const int i = tid - D / 4;
-      sm.new_v[i] = reinterpret_cast<const uint32_t*>(vn)[i];
-      sm.new_v[i + D / 4] = reinterpret_cast<const uint32_t*>(vn)[i + D / 4];
+
+  // ---- q: rotate, split; the new token ------------------------------------------------------------------------------------------
+  const float2 cs = reinterpret_cast<const float2*>(p.cos + (size_t)pos * (D / 2))[q_word], sn = reinterpret_cast<const float2*>(p.sin + (size_t)pos * (D / 2))[q_word];
+#pragma unroll
+  for (int i = 0; i < QI; ++i) {
+    const int r = q_row(i);
+    float z[2][2];  // [half][dim]
+    rotate(lo_f(q_lo[i]), lo_f(q_hi[i]), cs.x, sn.x, z[0][0], z[1][0]);
+    rotate(hi_f(q_lo[i]), hi_f(q_hi[i]), cs.y, sn.y, z[0][1], z[1][1]);
+    float most = fmaxf(fmaxf(fabsf(z[0][0]), fabsf(z[0][1])), fmaxf(fabsf(z[1][0]), fabsf(z[1][1])));
+#pragma unroll
+    for (int x = LPR / 2; x; x >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+    const int e = (int)(__float_as_uint(most) >> 23);  // biased exponent; 0 for a row of zeros, 255 for an infinity
+    // the largest element at 2^9 .. 2^10, after the factor that half of an e4m3 K's dims get
+    const int up = e == 0 || e == 255 ? 127 : min(254, 127 + (INT8 ? 9 : 1) + 127 - e);
+    const float mult = __uint_as_float((uint32_t)up << 23), to_f16 = !INT8 && (q_word & 2) ? mult * kLowE4m3 : mult;
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = r * S::QP + h * (D / 2) + 2 * q_word;
+      const __half2 hi = __floats2half2_rn(z[h][0] * to_f16, z[h][1] * to_f16);
+      const __half2 lo = __floats2half2_rn(z[h][0] * to_f16 - __low2float(hi), z[h][1] * to_f16 - __high2float(hi));
+      *reinterpret_cast<__half2*>(&sm.qh[at]) = hi;
+      *reinterpret_cast<__half2*>(&sm.ql[at]) = lo;
+      sum += (__low2float(hi) + __low2float(lo)) + (__high2float(hi) + __high2float(lo));
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const uint32_t part = pack_bf16(z[h][0], z[h][1]);
+        *reinterpret_cast<uint32_t*>(&sm.qb[k][at]) = part;
+        z[h][0] -= lo_f(part);
+        z[h][1] -= hi_f(part);
+      }
+    }
+    if constexpr (INT8) {
+#pragma unroll
+      for (int x = LPR / 2; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    }
+    if (q_word == 0) {
+      sm.qs[r] = p.scale * kLog2e / mult;
+      sm.qc[r] = 128.f * sum * (p.scale * kLog2e / mult);
     }
   }
+  if (owns_tail) store_new<D>(p, fresh, pos, sm.new_k, sm.new_v);
   if (tid == 0) sm.bad = 0;
   __syncthreads();
 
   // ---- state of the softmax: column 2t and 2t + 1 of each tile of eight queries ---------------------------------------------------
-  float o[NT][NM][4], m[NT][2], l[NT][2], f[NT][2];
+  float o[NT][NM][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int a = 0; a < NT; ++a) {
 #pragma unroll
@@ -291,163 +465,278 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) decode_attention8_k
     for (int h = 0; h < 2; ++h) {
       m[a][h] = -INFINITY;
       l[a][h] = 0.f;
-      f[a][h] = sm.qs[a * 8 + 2 * t + h];
     }
   }
 
-  // ---- the tail, one position per warp at a time: lanes share the dims -------------------------------------------------------------
-  if (owns_tail) {
-    constexpr int E = D / 32;  // dims of a lane
-    if (tile == 0 && tid < D / 2) {  // append; nobody reads this place before the next launch
-      reinterpret_cast<uint32_t*>(c.k_tail + tail_at + (size_t)place * D)[tid] = sm.new_k[tid];
-      reinterpret_cast<uint32_t*>(c.v_tail + tail_at + (size_t)place * D)[tid] = sm.new_v[tid];
-    }
-    float to[R][E], tm[R], tl[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      tm[r] = -INFINITY;
-      tl[r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) to[r][i] = 0.f;
-    }
-    for (int j = warp; j <= place; j += kWarps) {
-      const uint32_t* kp = j == place ? sm.new_k : reinterpret_cast<const uint32_t*>(c.k_tail + tail_at + (size_t)j * D);
-      const uint32_t* vp = j == place ? sm.new_v : reinterpret_cast<const uint32_t*>(c.v_tail + tail_at + (size_t)j * D);
-      float kk[E], vv[E];
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const uint32_t kw = kp[lane * (E / 2) + i], vw = vp[lane * (E / 2) + i];
-        kk[2 * i] = lo_f(kw), kk[2 * i + 1] = hi_f(kw);
-        vv[2 * i] = lo_f(vw), vv[2 * i + 1] = hi_f(vw);
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r >= rows) break;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) s += sm.qf[r * D + lane * E + i] * kk[i];
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= p.scale * kLog2e;
-        const float mn = fmaxf(tm[r], s);
-        const float corr = exp2_fast(tm[r] - mn), w = exp2_fast(s - mn);
-        tl[r] = tl[r] * corr + w;
-#pragma unroll
-        for (int i = 0; i < E; ++i) to[r][i] = to[r][i] * corr + w * vv[i];
-        tm[r] = mn;
-      }
-    }
-    // into the layout of the products, through this warp's part of shared memory
-    const float up = 256.f;  // 2^kHead
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) sm.o[warp][r * S::OP + lane * E + i] = to[r][i] * up;
-      if (lane == 0) {
-        sm.m[warp][r] = tm[r] - kHead;
-        sm.l[warp][r] = tl[r] * up;
-      }
-    }
-    __syncwarp();
-#pragma unroll
-    for (int a = 0; a < NT; ++a) {
-#pragma unroll
-      for (int i = 0; i < NM; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[a][i][e] = sm.o[warp][(a * 8 + 2 * t + (e & 1)) * S::OP + g * (D / 8) + 2 * i + (e >> 1)];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m[a][h] = sm.m[warp][a * 8 + 2 * t + h];
-        l[a][h] = g == 0 ? sm.l[warp][a * 8 + 2 * t + h] : 0.f;
-      }
-    }
-    __syncwarp();
-  }
-
-  // ---- the pages -----------------------------------------------------------------------------------------------------------------
-  float ks = 1.f, lvs = 0.f, ivs = 1.f;  // of the window's lane
-  for (int n = 0; n < n_units; ++n) {
-    if ((n & 31) == 0) {
-      ks = ks_next;
-      lvs = log2f(vs_next);
-      ivs = __frcp_rn(vs_next);
-    }
-    float s[NT][4], s2[NT][4];
+  // Scores (rows: positions g, g + 8 of each unit; columns: queries) into weights. Moves the references where a score passes them by kRoom.
+  auto weigh = [&](auto& s, const float* over_v) {
+    constexpr int H = sizeof(s[0]) / sizeof(s[0][0]);
+    bool over = false;
+    float top[NT][2];
 #pragma unroll
     for (int a = 0; a < NT; ++a)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[a][e] = s2[a][e] = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        top[a][e] = fmaxf(s[a][0][e], s[a][0][e + 2]);
 #pragma unroll
-    for (int j = 0; j < KJ; ++j) {
-      const uint32_t r0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w}, r8[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a0, a1, a2, a3;
-        widen<INT8>(r0[w], a0, a2);
-        widen<INT8>(r8[w], a1, a3);
-#pragma unroll
-        for (int a = 0; a < NT; ++a) {
-          const int q = (a * 8 + g) * S::QP + j * 64 + t * 16 + w * 4;
-          const uint2 h = *reinterpret_cast<const uint2*>(&sm.qh[q]), lo = *reinterpret_cast<const uint2*>(&sm.ql[q]);
-          mma(s[a], a0, a1, a2, a3, h.x, h.y);
-          mma(s2[a], a0, a1, a2, a3, lo.x, lo.y);
-        }
+        for (int h = 1; h < H; ++h) top[a][e] = fmaxf(top[a][e], fmaxf(s[a][h][e], s[a][h][e + 2]));
+        over = over || top[a][e] - m[a][e] > kRoom;
       }
-    }
-    load_k(n + 1);
-    const float uks = __shfl_sync(0xffffffffu, ks, n & 31), ulv = __shfl_sync(0xffffffffu, lvs, n & 31), uiv = __shfl_sync(0xffffffffu, ivs, n & 31);
-    bool over = false;
-#pragma unroll
-    for (int a = 0; a < NT; ++a) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[a][e] = (s[a][e] + s2[a][e]) * (f[a][e & 1] * uks) + ulv;
-      over = over || fmaxf(s[a][0], s[a][2]) - m[a][0] > kRoom || fmaxf(s[a][1], s[a][3]) - m[a][1] > kRoom;
-    }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
       for (int a = 0; a < NT; ++a)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(s[a][h], s[a][h + 2]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          if (top - m[a][h] > kRoom) {
-            const float corr = exp2_fast(m[a][h] - (top - kHead));
-            m[a][h] = top - kHead;
-            l[a][h] *= corr;
+        for (int e = 0; e < 2; ++e) {
+          float t0 = top[a][e];
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 4));
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 8));
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 16));
+          if (t0 - m[a][e] > kRoom) {
+            const float corr = exp2_fast(m[a][e] - (t0 - kHead));
+            m[a][e] = t0 - kHead;
+            l[a][e] *= corr;
 #pragma unroll
             for (int i = 0; i < NM; ++i) {
-              o[a][i][h] *= corr;
-              o[a][i][h + 2] *= corr;
+              o[a][i][e] *= corr;
+              o[a][i][e + 2] *= corr;
             }
           }
         }
     }
-    uint32_t b0[NT], b1[NT];
 #pragma unroll
-    for (int a = 0; a < NT; ++a) {
-      const float w0 = exp2_fast(s[a][0] - m[a][0]), w1 = exp2_fast(s[a][1] - m[a][1]);
-      const float w2 = exp2_fast(s[a][2] - m[a][0]), w3 = exp2_fast(s[a][3] - m[a][1]);
-      l[a][0] += (w0 + w2) * uiv;
-      l[a][1] += (w1 + w3) * uiv;
-      b0[a] = transpose8x8(pack_f16(w0, w1));
-      b1[a] = transpose8x8(pack_f16(w2, w3));
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[a][h][e] = exp2_fast(s[a][h][e] - m[a][e & 1]);
+        l[a][0] += (s[a][h][0] + s[a][h][2]) * over_v[h];
+        l[a][1] += (s[a][h][1] + s[a][h][3]) * over_v[h];
+      }
+  };
+
+  // ---- the pages -----------------------------------------------------------------------------------------------------------------
+  float f[NT][2], off[NT][2];
+#pragma unroll
+  for (int a = 0; a < NT; ++a)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      f[a][e] = sm.qs[a * 8 + 2 * t + e] * (INT8 ? kLowInt8 : 1.f);
+      off[a][e] = INT8 ? sm.qc[a * 8 + 2 * t + e] : 0.f;
     }
+  // K of pair n -> its products with q (two sums, which join later).
+  auto scores = [&](int n, float (&s)[2][NT][2][4]) {
+    const uint8_t* stage = &sm.ring[warp][0][0][0] + (n % kStages) * 4 * S::kUnit;
 #pragma unroll
-    for (int w = 0; w < VW; ++w) {
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][a][0][e] = s[0][a][1][e] = s[1][a][0][e] = s[1][a][1][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+      uint4 x[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t a0, a1, a2, a3;
-        widen<INT8>(__byte_perm(vr[0][w], vr[1][w], h ? 0x7362 : 0x5140), a0, a1);
-        widen<INT8>(__byte_perm(vr[2][w], vr[3][w], h ? 0x7362 : 0x5140), a2, a3);
+        const uint4* kr = reinterpret_cast<const uint4*>(stage + h * S::kUnit) + lane;
+        x[h][0] = kr[j * 64];
+        x[h][1] = kr[j * 64 + 32];
+      }
 #pragma unroll
-        for (int a = 0; a < NT; ++a) mma(o[a][2 * w + h], a0, a1, a2, a3, b0[a], b1[a]);
+      for (int w = 0; w < 4; ++w) {
+        uint32_t a0[2], a1[2], a2[2], a3[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t r0 = w == 0 ? x[h][0].x : (w == 1 ? x[h][0].y : (w == 2 ? x[h][0].z : x[h][0].w));
+          const uint32_t r8 = w == 0 ? x[h][1].x : (w == 1 ? x[h][1].y : (w == 2 ? x[h][1].z : x[h][1].w));
+          if constexpr (INT8) {
+            widen_int8_low(r0, a0[h], a2[h]);
+            widen_int8_low(r8, a1[h], a3[h]);
+          } else if (w & 1) {
+            widen_e4m3_low(r0, a0[h], a2[h]);
+            widen_e4m3_low(r8, a1[h], a3[h]);
+          } else {
+            widen_e4m3(r0, a0[h], a2[h]);
+            widen_e4m3(r8, a1[h], a3[h]);
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+          const int q = (a * 8 + g) * S::QP + j * 64 + t * 16 + w * 4;
+          const uint2 hi = *reinterpret_cast<const uint2*>(&sm.qh[q]), lo = *reinterpret_cast<const uint2*>(&sm.ql[q]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            mma(s[0][a][h], a0[h], a1[h], a2[h], a3[h], hi.x, hi.y);
+            mma(s[1][a][h], a0[h], a1[h], a2[h], a3[h], lo.x, lo.y);
+          }
+        }
       }
     }
-    load_v(n + 1);
+  };
+  // The scores of the pair after the next are not asked for before K of the next one is read, and so on: while the weights and values of
+  // pair n go their way (exponentials, transposes, products one after the other), the products of pair n + 1 have nothing to wait for.
+  // In the order of asking: .. K(n + 1) V(n) | K(n + 2) V(n + 1): two more than are waited for.
+  float ks = 1.f, lvs = 0.f, ivs = 1.f;  // of the window's lane
+  float acc[2][NT][2][4];
+  size_t where[2] = {0, 0};  // of pair n + 2, whose V is still to be asked for
+  wait_copies<2 * kStages - 1>();
+  if (n_pairs > 0) {
+    scores(0, acc);
+    load_k(kStages, where);
+  } else {
+    copies_done();
   }
+  int n = 0;
+  for (; n < n_pairs; ++n) {
+    if ((n & 15) == 0) {
+      ks = ks_next;
+      lvs = log2f(vs_next);
+      ivs = __frcp_rn(vs_next);
+    }
+    float s[NT][2][4], uiv[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int src = 2 * (n & 15) + h;
+      const float uks = __shfl_sync(0xffffffffu, ks, src), ulv = __shfl_sync(0xffffffffu, lvs, src);
+      uiv[h] = __shfl_sync(0xffffffffu, ivs, src);
+      const bool there = unit_of(n, h) < units;
+#pragma unroll
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float rest = INT8 ? ulv - off[a][e & 1] * uks : ulv;
+          s[a][h][e] = (acc[0][a][h][e] + acc[1][a][h][e]) * (f[a][e & 1] * uks) + rest;
+          if (h == 1 && !there) s[a][h][e] = -INFINITY;
+        }
+    }
+    wait_copies<2>();
+    size_t next[2] = {0, 0};
+    if (n + 1 < n_pairs) {
+      scores(n + 1, acc);
+      load_k(n + 1 + kStages, next);  // where K(n + 1) was
+    } else {
+      copies_done();
+    }
+    weigh(s, uiv);
+    uint32_t b0[NT][2], b1[NT][2];
+#pragma unroll
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        b0[a][h] = transpose8x8(pack_f16(s[a][h][0], s[a][h][1]));
+        b1[a][h] = transpose8x8(pack_f16(s[a][h][2], s[a][h][3]));
+      }
+    const uint8_t* stage = &sm.ring[warp][0][0][0] + (n % kStages) * 4 * S::kUnit;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t vr[4][VW];
+      const uint8_t* vp = stage + (2 + h) * S::kUnit + v_place;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (VW == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vp + i * 512);
+          vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(vp + i * 256);
+          vr[i][0] = x.x, vr[i][1] = x.y;
+        }
+        if constexpr (INT8) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vr[i][w] ^= 0x80808080u;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t a0, a1, a2, a3;
+          const uint32_t y = __byte_perm(vr[0][w], vr[1][w], x ? 0x7362 : 0x5140), z = __byte_perm(vr[2][w], vr[3][w], x ? 0x7362 : 0x5140);
+          if constexpr (INT8) {
+            widen_biased(y, a0, a1);
+            widen_biased(z, a2, a3);
+          } else {
+            widen_e4m3(y, a0, a1);
+            widen_e4m3(z, a2, a3);
+          }
+#pragma unroll
+          for (int a = 0; a < NT; ++a) mma(o[a][2 * w + x], a0, a1, a2, a3, b0[a][h], b1[a][h]);
+        }
+      }
+    }
+    load_v(n + kStages, where);
+    where[0] = next[0];
+    where[1] = next[1];
+  }
+
+  // ---- the tail, q in three bf16 parts and the weights in two ------------------------------------------------------------------------
+  const float fs = p.scale * kLog2e;
+  for (; n < n_all; ++n) {
+    const int first = tail_first(n);
+    const uint4* stage = reinterpret_cast<const uint4*>(&sm.ring[warp][0][0][0] + (n % kStages) * 4 * S::kUnit) + lane;
+    float s[NT][1][4];
+#pragma unroll
+    for (int a = 0; a < NT; ++a) s[a][0][0] = s[a][0][1] = s[a][0][2] = s[a][0][3] = 0.f;
+    wait_copies<2>();
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint4 x0 = *(first + g == place ? sm.new_k + j * 4 + t : stage + j * 64);
+      const uint4 x8 = *(first + g + 8 == place ? sm.new_k + j * 4 + t : stage + j * 64 + 32);
+      const uint32_t r0[4] = {x0.x, x0.y, x0.z, x0.w}, r8[4] = {x8.x, x8.y, x8.z, x8.w};
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int i = 2; i >= 0; --i) {  // the small parts first
+            const uint2 q = *reinterpret_cast<const uint2*>(&sm.qb[i][(a * 8 + g) * S::QP + j * 32 + t * 8 + w * 4]);
+            mma_bf16(s[a][0], r0[2 * w], r8[2 * w], r0[2 * w + 1], r8[2 * w + 1], q.x, q.y);
+          }
+    }
+    load_k(n + kStages, where);
+#pragma unroll
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[a][0][e] = first + g + (e >> 1) * 8 <= place ? s[a][0][e] * fs : -INFINITY;
+    const float one[1] = {1.f};
+    weigh(s, one);
+    // two bf16 parts of the weights, the upper half of their bits and the rest, which is never zero: an infinity stays one
+    uint32_t b0[2][NT], b1[2][NT];
+    auto rest = [](float w) { return fmaxf(w - __uint_as_float(__float_as_uint(w) & 0xffff0000u), 7.5231638e-37f); };
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+      const float* w = s[a][0];
+      b0[0][a] = transpose8x8(__byte_perm(__float_as_uint(w[0]), __float_as_uint(w[1]), 0x7632));
+      b1[0][a] = transpose8x8(__byte_perm(__float_as_uint(w[2]), __float_as_uint(w[3]), 0x7632));
+      b0[1][a] = transpose8x8(pack_bf16(rest(w[0]), rest(w[1])));
+      b1[1][a] = transpose8x8(pack_bf16(rest(w[2]), rest(w[3])));
+    }
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      uint4 v[4];  // zeros behind the new position
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = *(first + 2 * t + (i & 1) + (i >> 1) * 8 == place ? sm.new_v + g * (D / 64) + j : stage + 2 * S::kUnit / 16 + (i * (D / 64) + j) * 32);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        auto word = [&](int i) { return w == 0 ? v[i].x : (w == 1 ? v[i].y : (w == 2 ? v[i].z : v[i].w)); };
+        const uint32_t a0 = __byte_perm(word(0), word(1), 0x5410), a1 = __byte_perm(word(0), word(1), 0x7632);
+        const uint32_t a2 = __byte_perm(word(2), word(3), 0x5410), a3 = __byte_perm(word(2), word(3), 0x7632);
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+          mma_bf16(o[a][j * 4 + w], a0, a1, a2, a3, b0[1][a], b1[1][a]);
+          mma_bf16(o[a][j * 4 + w], a0, a1, a2, a3, b0[0][a], b1[0][a]);
+        }
+      }
+    }
+    load_v(n + kStages, where);
+  }
+  wait_copies<0>();
+  if (owns_tail && tile == 0)
+    if (tid < D / 4) {  // append; nobody reads this place before the next launch
+      const int i = tid % (D / 8);
+      __nv_bfloat16* to = (tid < D / 8 ? c.k_tail : c.v_tail) + tail_at + (size_t)place * D;
+      reinterpret_cast<uint4*>(to)[i] = (tid < D / 8 ? sm.new_k : sm.new_v)[i];
+    }
   if (bad) sm.bad = 1;
+
+  __syncthreads();  // the rings and q are not needed any more
 
   // ---- join the warps --------------------------------------------------------------------------------------------------------------
 #pragma unroll
@@ -465,46 +754,74 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) decode_attention8_k
 #pragma unroll
     for (int i = 0; i < NM; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sm.o[warp][(a * 8 + 2 * t + (e & 1)) * S::OP + g * (D / 8) + 2 * i + (e >> 1)] = o[a][i][e];
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<float2*>(&sm.o[warp][(a * 8 + 2 * t + e) * S::OP + g * S::OS + 2 * i]) = make_float2(o[a][i][e], o[a][i][e + 2]);
   }
   __syncthreads();
   const bool any_bad = sm.bad != 0;
-  for (int r = tid / D; r < rows; r += kThreads / D) {
-    const int d = tid & (D - 1);
+  constexpr int PR = D / 2;  // pairs of dims of a row
+  static_assert(kThreads % PR == 0 || PR % kThreads == 0, "whole rows");
+#pragma unroll 4
+  for (int i = tid; i < rows * PR; i += kThreads) {
+    const int r = i / PR, d = 2 * (i % PR);
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][r]);
-    float L = 0.f, acc = 0.f;
+    float L = 0.f, x0 = 0.f, x1 = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float x = sm.m[w][r] == -INFINITY ? 0.f : exp2_fast(sm.m[w][r] - M);
+      const float2 v = *reinterpret_cast<const float2*>(&sm.o[w][r * S::OP + d / (D / 8) * S::OS + d % (D / 8)]);
       L += sm.l[w][r] * x;
-      acc += sm.o[w][r * S::OP + d] * x;
+      x0 += v.x * x;
+      x1 += v.y * x;
     }
     if (sp.used == 1) {
-      out[(size_t)r * D + d] = __float2bfloat16(any_bad ? 0.f : acc / L);
+      const float inv = 1.f / L;
+      reinterpret_cast<uint32_t*>(out + (size_t)r * D)[d / 2] = any_bad ? 0 : pack_bf16(x0 * inv, x1 * inv);
+    } else if (p.cluster) {
+      sm.joined[r * (PR + 1) + d / 2] = make_float2(x0, x1);
+      if (d == 0) sm.joined[r * (PR + 1) + PR] = make_float2(any_bad ? INFINITY : M, L);
     } else {
       float* part = p.partials + (((size_t)b * p.n_heads + head0 + r) * p.nsplit + split) * (D + 2);
-      part[2 + d] = acc;
-      if (d == 0) {
-        part[0] = any_bad ? INFINITY : M;
-        part[1] = L;
+      *reinterpret_cast<float2*>(part + 2 + d) = make_float2(x0, x1);
+      if (d == 0) *reinterpret_cast<float2*>(part) = make_float2(any_bad ? INFINITY : M, L);
+    }
+  }
+  if (sp.used == 1 || !p.cluster) return;
+  // ---- join the splits, which are the CTAs of the cluster (those without work have left): each takes its share of the rows -------------
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  for (int i = split * kThreads + tid; i < rows * PR; i += sp.used * kThreads) {
+    const int r = i / PR, at = r * (PR + 1);
+    const uint32_t out_at = ptx::smem_u32(&sm.joined[at + i % PR]), ml_at = ptx::smem_u32(&sm.joined[at + PR]);
+    float2 ml[kMaxCluster], x[kMaxCluster];
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k)
+      if (k < sp.used) {
+        ml[k] = ld_cluster(ptx::mapa(ml_at, k));
+        x[k] = ld_cluster(ptx::mapa(out_at, k));
       }
-    }
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k)
+      if (k < sp.used) M = fmaxf(M, ml[k].x);
+    float L = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k)
+      if (k < sp.used) {
+        const float w = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - M);
+        L += ml[k].y * w;
+        x0 += x[k].x * w;
+        x1 += x[k].y * w;
+      }
+    reinterpret_cast<uint32_t*>(out + (size_t)r * D)[i % PR] = M == INFINITY ? 0 : pack_bf16(x0 / L, x1 / L);
   }
-
-  // ---- the block is full: quantise it ------------------------------------------------------------------------------------------------
-  if (owns_tail && tile == 0 && place == c.block - 1) {
-    const int page = table[pos / c.block];
-    if ((unsigned)page < (unsigned)c.num_blocks) {
-      const size_t at8 = ((size_t)page * c.n_kv_heads + kvh) * c.block * D, sc = (size_t)page * c.n_kv_heads + kvh;
-      quantise_block<D, INT8>(c.k_tail + tail_at, sm.new_k, c.block, sm.amax[0], c.k + at8, c.k_scale + sc);
-      quantise_block<D, INT8>(c.v_tail + tail_at, sm.new_v, c.block, sm.amax[1], c.v + at8, c.v_scale + sc);
-    }
-  }
+  ptx::cluster_arrive();  // nobody leaves while its results are read
+  ptx::cluster_wait();
 }
 
-// Joins the splits of a sequence that has more than one.
+// Joins the splits of a sequence that has more than one, where they are too many for a cluster.
 template <int D>
 __global__ void __launch_bounds__(D) merge_splits_kernel(const DecodeAttn8Params p) {
   ptx::griddep_launch_dependents();
@@ -512,7 +829,7 @@ __global__ void __launch_bounds__(D) merge_splits_kernel(const DecodeAttn8Params
   const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
   const int pos = p.positions[b];
   if (!position_ok(p, pos)) return;
-  const int used = split_of(pos, p.cache.block, p.nsplit).used;
+  const int used = split_of(pos, p).used;
   if (used == 1) return;
   const float* part = p.partials + ((size_t)b * p.n_heads + h) * p.nsplit * (D + 2);
   float M = -INFINITY;
@@ -534,25 +851,37 @@ cudaError_t launch(const DecodeAttn8Params& p, cudaStream_t stream) {
   static DeviceOnce configured;
   if (configured.pending()) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     configured.done();
   }
-  const int group = p.n_heads / p.cache.n_kv_heads;
+  const int group = p.n_heads / p.cache.n_kv_heads, tiles = (group + 8 * NT - 1) / (8 * NT);
+  const long long pairs = (long long)p.batch * p.cache.n_kv_heads * tiles, quantisers = (long long)p.batch * p.cache.n_kv_heads;
+  const long long ctas = (pairs + (quantisers + p.nsplit - 1) / p.nsplit) * p.nsplit;
+  if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.nsplit, p.cache.n_kv_heads * ((group + 8 * NT - 1) / (8 * NT)), p.batch);
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sizeof(Smem<D, NT>);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
   cfg.numAttrs = pdl_launch_attr(&attr[0]);
+  if (p.cluster) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = p.nsplit;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return e;
   launch_count_add(1);
-  if (p.nsplit == 1) return cudaSuccess;
+  if (p.nsplit == 1 || p.cluster) return cudaSuccess;
   cfg.gridDim = dim3(p.n_heads, p.batch);
   cfg.blockDim = dim3(D);
   cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = pdl_launch_attr(&attr[0]);
   e = cudaLaunchKernelEx(&cfg, merge_splits_kernel<D>, p);
   if (e == cudaSuccess) launch_count_add(1);
   return e;
@@ -570,17 +899,23 @@ bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 
 
 }  // namespace
 
-int decode_attention8_splits(const DecodeAttn8Params& p) {
+void decode_attention8_split(DecodeAttn8Params& p) {
   const int group = p.n_heads / p.cache.n_kv_heads;
-  const int r = group > 8 ? 16 : 8;
+  const int r = group > 8 ? 16 : 8, places = (group > 8 ? 2 : 3) * 148;  // query rows of a CTA, and CTAs that the GPU holds at a time
   const long long pairs = (long long)p.batch * p.cache.n_kv_heads * ((group + r - 1) / r);
-  // about four CTAs for every place (four on an SM), so that sequences of different lengths even out, of at least kMinUnits units
-  const long long cap = ((long long)p.max_blocks * (p.cache.block / 16) + kMinUnits - 1) / kMinUnits;
-  return (int)std::max(1ll, std::min({4ll * 4 * 148 / std::max(1ll, pairs), cap, 64ll}));
+  const long long units = (long long)p.max_blocks * (p.cache.block / 16);  // at most; how long the sequences are only the GPU knows
+  // As many CTAs as the GPU holds at a time, or, where there are more pairs than that, splits of kChunk units; none shorter than kLeast.
+  const long long want = pairs <= places ? places / pairs : (units + kChunk - 1) / kChunk;
+  p.nsplit = (int)std::max(1ll, std::min({want, (long long)kMaxSplits, (units + kLeast - 1) / kLeast}));
+  p.least = pairs <= places ? kLeast : kChunk;
+  // The CTAs of a sequence are a cluster, which joins their results without a second launch, unless there is so much for so few heads
+  // that more of them pay.
+  if (p.nsplit > kMaxCluster && units <= kMaxCluster * 64) p.nsplit = kMaxCluster;
+  p.cluster = p.nsplit > 1 && p.nsplit <= kMaxCluster;
 }
 
 size_t decode_attention8_partial_floats(const DecodeAttn8Params& p) {
-  return p.nsplit > 1 ? (size_t)p.batch * p.n_heads * p.nsplit * (p.cache.head_dim + 2) : 0;
+  return p.nsplit > 1 && !p.cluster ? (size_t)p.batch * p.n_heads * p.nsplit * (p.cache.head_dim + 2) : 0;
 }
 
 cudaError_t decode_attention8(const DecodeAttn8Params& p, cudaStream_t stream) {
@@ -588,7 +923,7 @@ cudaError_t decode_attention8(const DecodeAttn8Params& p, cudaStream_t stream) {
   if (p.batch == 0) return cudaSuccess;
   if (p.batch < 0 || p.batch > 65535 || p.nsplit < 1 || c.n_kv_heads < 1 || p.n_heads < 1 || p.n_heads % c.n_kv_heads != 0 || p.n_heads > 65535) return cudaErrorInvalidValue;
   if (c.block < 16 || c.block > 128 || (c.block & (c.block - 1)) != 0 || p.max_blocks < 1 || c.requests < p.batch) return cudaErrorInvalidValue;
-  if (p.nsplit > 1 && !p.partials) return cudaErrorInvalidValue;
+  if (p.nsplit > 1 && !p.cluster && !p.partials) return cudaErrorInvalidValue;
   if (!aligned16(p.qkv) || !aligned16(c.k) || !aligned16(c.v) || !aligned16(c.k_tail) || !aligned16(c.v_tail) || !aligned16(p.out)) return cudaErrorInvalidValue;
   if (p.qkv_stride % 8 != 0 || p.out_stride % 8 != 0) return cudaErrorInvalidValue;
   if (c.head_dim == 128) return by_tile<128>(p, stream);

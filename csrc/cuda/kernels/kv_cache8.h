@@ -56,12 +56,14 @@ struct DecodeAttn8Params {
   __nv_bfloat16* out;        // [batch, out_stride]
   long long out_stride;
   float* partials;           // decode_attention8_partial_floats() floats; unused when there is one split
-  int batch, n_heads, max_blocks, table_rows, nsplit;
+  int batch, n_heads, max_blocks, table_rows;
+  int nsplit, least;  // set by decode_attention8_split()
+  bool cluster;
   float scale;               // 1 / sqrt(head_dim)
   KvCache8 cache;
 };
-int decode_attention8_splits(const DecodeAttn8Params& p);
-size_t decode_attention8_partial_floats(const DecodeAttn8Params& p);  // with p.nsplit set
+void decode_attention8_split(DecodeAttn8Params& p);
+size_t decode_attention8_partial_floats(const DecodeAttn8Params& p);  // with the split set
 cudaError_t decode_attention8(const DecodeAttn8Params& p, cudaStream_t stream);
 
 }  // namespace ccl
