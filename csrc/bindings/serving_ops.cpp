@@ -4,6 +4,8 @@
 // tracing refuses what a launch would refuse.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <torch/torch.h>
 
@@ -448,6 +450,40 @@ Tensor token_logprobs_backward_meta(const Tensor& logits, const Tensor& targets,
   return at::empty_strided({logits.size(0), vocab}, {vocab + ((row_stride(logits) - vocab) % per + per) % per, 1}, logits.options());
 }
 
+// The gradient of the whole-vocabulary form (a Python function does as much, for about 20 us more of the host's time a step).
+class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& targets, int64_t top) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ccl::token_logprobs", "").typed<Logprobs(const Tensor&, const Tensor&, int64_t)>();
+    auto [logprob, entropy, lse, top_logprobs, top_ids] = op.call(logits, targets, top);
+    ctx->save_for_backward({logits, targets, lse, entropy, top_ids});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({lse, top_ids});
+    return {logprob, entropy, lse, top_logprobs, top_ids};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+    auto given = [&](int i) { return grads[i].defined() ? optional<Tensor>(grads[i].contiguous()) : optional<Tensor>(); };
+    const auto g_lp = given(0), g_ent = given(1), g_top = given(3);
+    if (!g_lp && !g_ent && !g_top) return {Tensor(), Tensor(), Tensor()};
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("ccl::token_logprobs_backward", "")
+                         .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const optional<Tensor>&,
+                                       const optional<Tensor>&, int64_t, int64_t)>();
+    const auto s = ctx->get_saved_variables();
+    return {op.call(s[0], s[1], s[2], s[3], s[4], g_lp, g_ent, g_top, 0, s[0].size(1)), Tensor(), Tensor()};
+  }
+};
+Logprobs token_logprobs_autograd(const Tensor& logits, const Tensor& targets, int64_t top) {
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    auto out = TokenLogprobs::apply(logits, targets, top);
+    return {out[0], out[1], out[2], out[3], out[4]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ccl::token_logprobs", "").typed<Logprobs(const Tensor&, const Tensor&, int64_t)>();
+  return op.call(logits, targets, top);
+}
+
 }  // namespace
 
 #define CACHE_SCHEMA "Tensor(a!) k, Tensor(b!) v, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor(e!) k_tail, Tensor(f!) v_tail, Tensor cos, Tensor sin, int n_heads"
@@ -490,4 +526,9 @@ TORCH_LIBRARY_IMPL(ccl, Meta, m) {
   m.impl("token_logprobs_shard", &token_logprobs_shard_meta);
   m.impl("token_logprobs_merge", &token_logprobs_merge_meta);
   m.impl("token_logprobs_backward", &token_logprobs_backward_meta);
+}
+
+TORCH_LIBRARY_IMPL(ccl, Autograd, m) {
+  m.impl("token_logprobs", &token_logprobs_autograd);
+  m.impl("token_logprobs_backward", torch::autograd::autogradNotImplementedFallback());  // a second derivative is an error, not zero
 }

@@ -2,15 +2,16 @@
 //
 // Forward. A thread keeps a reference m, sum e^(x - m) and sum e^(x - m) (x - m); they join into log sum exp and the entropy
 // H = log s - t / s. The reference is raised only when a value passes it by more than kLag, so the loop has no dependent maximum.
-// Bound by memory (one read of the logits) as long as the exponentials keep up: one per element, 16 a clock and SM.
+// Bound by memory (one read of the logits) in fp32, by instructions and the exponentials (16 a clock and SM) in 16 bits; so the
+// arithmetic is done two elements an instruction (f32x2).
 // A row belongs to one CTA; few rows are split over the CTAs of a cluster, which push their sums into the first one's shared memory.
 //
-// Alternatives. Nothing is sorted while the row streams by: every thread only remembers its largest value and the vector that it came from.
-// With K of these as (value, lowest index first) keys, the K-th largest over all threads is a bound that K elements of the row reach, and only
-// the threads whose own largest reaches it, exactly K of them, can hold an element that does. Those threads' elements (K out of 512
-// shares of the row) are read once more, from L2, into a sorted list per warp (lane i holds the i-th best), and the lists are joined
-// by counting for every candidate how many are better. Keys are unique, so the result does not depend on any order of execution, and
-// rows of equal or masked values cost no more than others.
+// Alternatives. Nothing is sorted while the row streams by: every thread only remembers its largest value and the vector that it came from,
+// as a key (value, lowest index first; keys are unique). The K-th largest of 64 groups' largest keys is a bound that K elements reach,
+// and only threads whose own key reaches it, about K of them, can hold an element that does. Their vectors (K of 512 shares of the row)
+// are read once more, from L2, one a thread, and what reaches the bound is put down in shared memory in any order: its place is the
+// number of better ones. If more reach the bound than there is room for (equal or sorted values), the K-th of those that were put down
+// is a better bound. The result does not depend on any order of execution.
 //
 // Values that are masked with -inf or with the type's lowest value take no part in the sums (0 * inf is not computed); a row with a NaN or
 // with +inf, or with nothing but -inf, has a NaN log-probability as log_softmax has.
@@ -21,13 +22,15 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cstring>
 
 namespace ccl {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLag = 6.f;
+constexpr float kLag = 8.f;
 constexpr int kMaxCluster = 16;
+constexpr int kClusterVecs = 1024;  // 16-byte vectors of a row for each CTA of its cluster, at least
 constexpr uint32_t kAbsent = 0xffffffffu;  // bits of "the target is in another shard"
 
 __device__ __forceinline__ float ex2(float x) {
@@ -52,28 +55,12 @@ __device__ __forceinline__ unsigned long long key_of(float x, uint32_t index) { 
 __device__ __forceinline__ float value_of(unsigned long long key) { return unordered((uint32_t)(key >> 32)); }
 __device__ __forceinline__ uint32_t index_of(unsigned long long key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ unsigned long long exchange(unsigned long long k, int x, bool larger) {
-  const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, x);
-  return (other > k) == larger ? other : k;
-}
-// Sorts a bitonic sequence over the lanes, largest first.
-__device__ __forceinline__ unsigned long long sort_bitonic(unsigned long long k, int lane) {
-#pragma unroll
-  for (int x = 16; x; x >>= 1) k = exchange(k, x, (lane & x) == 0);
-  return k;
-}
-__device__ __forceinline__ unsigned long long sort_warp(unsigned long long k, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int x = size >> 1; x; x >>= 1) k = exchange(k, x, ((lane & x) == 0) == ((lane & size) == 0));
-  return k;
-}
-// Puts `cand` (the same in all lanes) into the list that the lanes hold, largest first; the last one falls out.
-__device__ __forceinline__ void insert(unsigned long long& list, unsigned long long cand, int lane) {
-  const int at = __popc(__ballot_sync(0xffffffffu, list > cand));
-  const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
-  list = lane < at ? list : (lane == at ? cand : up);
+// How many of keys[0 .. n) are better than k.
+__device__ __forceinline__ int rank_of(const unsigned long long* keys, int n, unsigned long long k) {
+  int better = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) better += keys[i] > k;
+  return better;
 }
 
 // ---- sums -------------------------------------------------------------------------------------------------------------------------------
@@ -102,15 +89,76 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return a;
 }
 
+// The same in the loop over a row, where m is a whole number of powers of two: x log2 e - m is one multiply-add without an error in m, and sums
+// join exactly. A value that is masked (-inf, or the type's lowest) is raised to where its exponential is still zero but 0 * d is not NaN.
+// Rows that this does not hold for (nothing but masked values, infinities, NaN) are found by their sums and done again with Sums.
+struct FastSums {
+  float m, s, t;
+};
+__device__ __forceinline__ FastSums fast_nothing() { return {-FLT_MAX, 0.f, 0.f}; }
+__device__ __forceinline__ void rebase(FastSums& a, float m) {
+  const float delta = a.m - m, f = ex2(delta);
+  a.t = f * (a.t + delta * a.s);
+  a.s *= f;
+  a.m = m;
+}
+__device__ __forceinline__ void raise_to(FastSums& a, float most) {
+  if (fmaf(most, kLog2e, -a.m) > kLag) rebase(a, rintf(most * kLog2e));
+}
+__device__ __forceinline__ void add(FastSums& a, float x) {
+  const float d = fmaf(x, kLog2e, -a.m), e = ex2(d);
+  a.s += e;
+  a.t = fmaf(e, d, a.t);
+}
+__device__ __forceinline__ FastSums join(FastSums a, FastSums b) {
+  const float m = fmaxf(a.m, b.m);
+  rebase(a, m);
+  rebase(b, m);
+  a.s += b.s;
+  a.t += b.t;
+  return a;
+}
+// m to natural units; what its rounding leaves goes into the sums.
+__device__ __forceinline__ Sums natural(const FastSums& a) {
+  constexpr float kLn2High = 0.693145752f, kLn2Low = 1.42860677e-6f;  // the upper 16 bits of ln 2, and the rest
+  const float high = a.m * kLn2High, low = a.m * kLn2Low;             // (the first is exact for |m| up to 2^8)
+  const float m = high + low, left = (fmaf(a.m, kLn2High, -high) + (high - m)) + low;
+  const float f = 1.f + left + 0.5f * left * left;
+  return {m, a.s * f, fmaf(left * kLog2e, a.s, a.t) * f};
+}
+
+template <typename P>
+__device__ __forceinline__ P halves(uint32_t a) {
+  P p;
+  memcpy(&p, &a, 4);
+  return p;
+}
+template <typename P>
+__device__ __forceinline__ uint32_t bits(const P& p) {
+  uint32_t a;
+  memcpy(&a, &p, 4);
+  return a;
+}
+
 // ---- vectors of 16 bytes ------------------------------------------------------------------------------------------------------------------
 template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
+  static constexpr float kMasked = -1e37f, kLow = -1e30f;  // what masked values are raised to; below kLow a row's maximum makes it a special one
+  static __device__ __forceinline__ uint4 raised(const uint4& w) {
+    return make_uint4(__float_as_uint(max_nan(__uint_as_float(w.x), kMasked)), __float_as_uint(max_nan(__uint_as_float(w.y), kMasked)),
+                      __float_as_uint(max_nan(__uint_as_float(w.z), kMasked)), __float_as_uint(max_nan(__uint_as_float(w.w), kMasked)));
+  }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[4]) {
     x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    float x[N];
+    unpack(w, x);
+    return most(w, x);
   }
   static __device__ __forceinline__ float most(const uint4&, const float (&x)[4]) { return max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])); }
   static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
@@ -121,49 +169,62 @@ struct Vec<float> {
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
+  static constexpr float kMasked = -9.96921e36f, kLow = -1e30f;
+  static __device__ __forceinline__ uint4 raised(const uint4& w) {
+    const __nv_bfloat162 low = __float2bfloat162_rn(kMasked);
+    auto up = [&](uint32_t a) { return bits(__hmax2_nan(halves<__nv_bfloat162>(a), low)); };
+    return make_uint4(up(w.x), up(w.y), up(w.z), up(w.w));
+  }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[8]) {
     const uint32_t a[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(a[i] << 16), x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
   }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    const float unused[8] = {};
+    return most(w, unused);
+  }
   static __device__ __forceinline__ float most(const uint4& w, const float (&)[8]) {
-    const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(&w);
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(a[0], a[1]), __hmax2_nan(a[2], a[3]));
+    using P = __nv_bfloat162;
+    const P m = __hmax2_nan(__hmax2_nan(halves<P>(w.x), halves<P>(w.y)), __hmax2_nan(halves<P>(w.z), halves<P>(w.w)));
     return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-    uint4 w;
-    __nv_bfloat162* a = reinterpret_cast<__nv_bfloat162*>(&w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    return w;
+    return make_uint4(bits(__floats2bfloat162_rn(x[0], x[1])), bits(__floats2bfloat162_rn(x[2], x[3])), bits(__floats2bfloat162_rn(x[4], x[5])),
+                      bits(__floats2bfloat162_rn(x[6], x[7])));
   }
   static __device__ __forceinline__ __nv_bfloat16 to(float x) { return __float2bfloat16_rn(x); }
 };
 template <>
 struct Vec<__half> {
   static constexpr int N = 8;
+  static constexpr float kMasked = -65504.f, kLow = -3e4f;
+  static __device__ __forceinline__ uint4 raised(const uint4& w) {
+    const __half2 low = __float2half2_rn(kMasked);
+    auto up = [&](uint32_t a) { return bits(__hmax2_nan(halves<__half2>(a), low)); };
+    return make_uint4(up(w.x), up(w.y), up(w.z), up(w.w));
+  }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[8]) {
-    const __half2* a = reinterpret_cast<const __half2*>(&w);
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(a[i]);
+      const float2 f = __half22float2(halves<__half2>(a[i]));
       x[2 * i] = f.x, x[2 * i + 1] = f.y;
     }
   }
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    const float unused[8] = {};
+    return most(w, unused);
+  }
   static __device__ __forceinline__ float most(const uint4& w, const float (&)[8]) {
-    const __half2* a = reinterpret_cast<const __half2*>(&w);
-    const __half2 m = __hmax2_nan(__hmax2_nan(a[0], a[1]), __hmax2_nan(a[2], a[3]));
+    using P = __half2;
+    const P m = __hmax2_nan(__hmax2_nan(halves<P>(w.x), halves<P>(w.y)), __hmax2_nan(halves<P>(w.z), halves<P>(w.w)));
     return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-    uint4 w;
-    __half2* a = reinterpret_cast<__half2*>(&w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    return w;
+    return make_uint4(bits(__floats2half2_rn(x[0], x[1])), bits(__floats2half2_rn(x[2], x[3])), bits(__floats2half2_rn(x[4], x[5])), bits(__floats2half2_rn(x[6], x[7])));
   }
   static __device__ __forceinline__ __half to(float x) { return __float2half_rn(x); }
 };
@@ -194,19 +255,24 @@ __device__ __forceinline__ RowResult finish(const Sums& a, long long target, lon
   return r;
 }
 
+constexpr int kGroups = 64, kRoom = 512;
 template <int WARPS>
 struct FwdSmem {
+  FastSums fast[WARPS];
   Sums warp[WARPS];
-  Sums rank[kMaxCluster];                               // in the cluster's first CTA
-  unsigned long long lists[WARPS][32];                  // the threads' largest; later the warps' candidates
-  unsigned long long best[kMaxCluster][32];             // in the cluster's first CTA: candidates of each CTA
+  Sums rank[kMaxCluster];                          // in the cluster's first CTA
+  unsigned long long group[kGroups];               // the largest key of each group of threads
+  unsigned long long found[kRoom];                 // candidates
+  unsigned long long best[kMaxCluster][kMaxTopLogprobs];  // in the cluster's first CTA: the best of each CTA, in order
   unsigned long long bound;
-  int count[WARPS];
+  int n_threads, n_found;
+  uint16_t threads[WARPS * 32];                    // those that may hold a candidate
   float lse;
+  bool special;
 };
 
 template <typename T, int WARPS, bool TOP>
-__global__ void __launch_bounds__(WARPS * 32) token_logprobs_kernel(const LogprobParams p, int cluster) {
+__global__ void __launch_bounds__(WARPS * 32, 48 / WARPS) token_logprobs_kernel(const LogprobParams p, int cluster) {
   constexpr int N = Vec<T>::N, kThreads = WARPS * 32, U = 4;
   __shared__ FwdSmem<WARPS> sm;
   if (cluster > 1) ptx::cluster_arrive();  // the first CTA's shared memory is written to only after it has started
@@ -218,19 +284,20 @@ __global__ void __launch_bounds__(WARPS * 32) token_logprobs_kernel(const Logpro
   const int v0 = (int)((long long)sh.vecs * rank / cluster), v1 = (int)((long long)sh.vecs * (rank + 1) / cluster);
   const T* vec0 = row + sh.head;
 
-  Sums a = nothing();
+  FastSums a = fast_nothing();
   float top = 0.f;     // the thread's largest and the vector that it is in
   int top_vec = -1;
   auto take = [&](const uint4& w, int v) {
     float x[N];
-    Vec<T>::unpack(w, x);
-    const float most = Vec<T>::most(w, x);
-    if (!(most - a.m <= kLag)) {
-      if (TOP && (top_vec < 0 || most > top || (most != most && top == top))) top = most, top_vec = v;
-      rebase(a, most);
-    } else if (TOP && (top_vec < 0 || most > top)) {
-      top = most, top_vec = v;
+    const uint4 y = Vec<T>::raised(w);
+    Vec<T>::unpack(y, x);
+    const float most = Vec<T>::most(y, x);
+    if constexpr (TOP) {
+      // (equal to or below kMasked: the vector's own largest)
+      const float m = most <= Vec<T>::kMasked ? Vec<T>::largest(w) : most;
+      if (top_vec < 0 || m > top || (m != m && top == top)) top = m, top_vec = v;
     }
+    raise_to(a, most);
 #pragma unroll
     for (int i = 0; i < N; ++i) add(a, x[i]);
   };
@@ -252,94 +319,108 @@ __global__ void __launch_bounds__(WARPS * 32) token_logprobs_kernel(const Logpro
   float x_extra = 0.f;
   if (extra >= 0) {
     x_extra = Vec<T>::one(row + extra);
-    if (!(x_extra - a.m <= kLag)) rebase(a, x_extra);
-    add(a, x_extra);
+    const float x = max_nan(x_extra, Vec<T>::kMasked);
+    raise_to(a, x);
+    add(a, x);
   }
 
   // ---- alternatives of this CTA's share -----------------------------------------------------------------------------------------------------
   if constexpr (TOP) {
     const int K = p.top;
-    unsigned long long mine = top_vec >= 0 ? key_of(top, (uint32_t)top_vec) : 0;
-    unsigned long long k = sort_warp(mine, lane);
-    sm.lists[warp][lane] = k;
+    // a thread's key has the last element of the vector that its largest value is in, so that all of that vector's equal ones reach it
+    const unsigned long long mine = top_vec >= 0 ? key_of(top, (uint32_t)(sh.head + top_vec * N + N - 1)) : 0;
+    unsigned long long g = mine;
 #pragma unroll
-    for (int half = WARPS / 2; half; half >>= 1) {
-      __syncthreads();
-      if (warp < half) {
-        const unsigned long long other = sm.lists[warp + half][31 - lane];
-        k = sort_bitonic(k > other ? k : other, lane);
-        sm.lists[warp][lane] = k;
-      }
+    for (int x = kThreads / kGroups / 2; x; x >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, x);
+      g = other > g ? other : g;
     }
-    if (warp == 0 && lane == K - 1) sm.bound = k;
-    __syncthreads();
-    const unsigned long long bound = sm.bound;  // 0 when fewer than K threads have anything
-    unsigned long long list = 0;
-    auto offer = [&](unsigned long long cand) {  // 0: none
-      unsigned left;
-      while ((left = __ballot_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, list, K - 1)))) {
-        const int src = __ffs(left) - 1;
-        insert(list, __shfl_sync(0xffffffffu, cand, src), lane);
-        if (lane == src) cand = 0;
-      }
-    };
-    for (unsigned who = __ballot_sync(0xffffffffu, mine != 0 && mine >= bound); who; who &= who - 1) {
-      const int first = v0 + warp * 32 + __ffs(who) - 1;
-      for (int base = first; base < v1; base += 32 * kThreads) {
-        const int vi = base + lane * kThreads;
-        float x[N];
-        if (vi < v1) Vec<T>::unpack(ptx::ld_nc_v4(vec0 + (size_t)vi * N), x);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          // what is below the bound's value is no candidate
-          unsigned long long cand = vi < v1 ? key_of(x[i], (uint32_t)(sh.head + vi * N + i)) : 0;
-          if ((uint32_t)(cand >> 32) < (uint32_t)(bound >> 32)) cand = 0;
-          offer(cand);
-        }
-      }
-    }
-    if (rank == 0 && warp < 2) offer(extra >= 0 ? key_of(x_extra, (uint32_t)extra) : 0);
-    // the K best of the warps' lists: a candidate's place is the number of better ones
-    if (lane >= K) list = 0;
-    sm.lists[warp][lane] = list;  // (all have read `bound`; nobody reads the lists of the sort any more)
-    if (lane == 0) sm.count[warp] = 0;
-    __syncwarp();
-    if (lane < K && list == 0) atomicAdd(&sm.count[warp], 1);
-    __syncthreads();
+    if (tid % (kThreads / kGroups) == 0) sm.group[tid / (kThreads / kGroups)] = g;
+    if (tid == 0) sm.n_threads = sm.n_found = 0, sm.bound = 0;
     if (tid < kMaxTopLogprobs) sm.best[rank][tid] = 0;
     __syncthreads();
-    if (list != 0) {
-      int place = lane;  // better ones of its own list
-      for (int w = 0; w < WARPS; ++w) {
-        if (w == warp) continue;
-        const int n = K - sm.count[w];
-        for (int i = 0; i < n && sm.lists[w][i] > list; ++i) ++place;
+    if (tid < kGroups) {
+      const unsigned long long k = sm.group[tid];
+      if (k != 0 && rank_of(sm.group, kGroups, k) == K - 1) sm.bound = k;  // (0, with fewer than K groups that have anything)
+    }
+    __syncthreads();
+    unsigned long long bound = sm.bound;
+    if (mine != 0 && mine >= bound) sm.threads[atomicAdd(&sm.n_threads, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int each = (v1 - v0 + kThreads - 1) / kThreads, items = sm.n_threads * each;  // vectors of a thread, and of all these
+    int n;
+    while (true) {
+      auto put = [&](unsigned long long k) {
+        if (k >= bound) {
+          const int at = atomicAdd(&sm.n_found, 1);
+          if (at < kRoom) sm.found[at] = k;
+        }
+      };
+      if (extra >= 0) put(key_of(x_extra, (uint32_t)extra));
+      for (int i0 = tid; i0 < items; i0 += U * kThreads) {
+        int at[U];
+        uint4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * kThreads;
+          at[u] = i < items ? v0 + sm.threads[i / each] + i % each * kThreads : v1;
+          if (at[u] < v1) w[u] = ptx::ld_nc_v4(vec0 + (size_t)at[u] * N);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (at[u] >= v1 || ordered(Vec<T>::largest(w[u])) < (uint32_t)(bound >> 32)) continue;
+          float x[N];
+          Vec<T>::unpack(w[u], x);
+#pragma unroll
+          for (int e = 0; e < N; ++e) put(key_of(x[e], (uint32_t)(sh.head + at[u] * N + e)));
+        }
       }
-      if (place < K) sm.best[rank][place] = list;
+      __syncthreads();
+      n = sm.n_found;
+      if (n <= kRoom) break;
+      // more than there is room for: the K-th best of those that found room, and again
+      for (int i = tid; i < kRoom; i += kThreads)
+        if (rank_of(sm.found, kRoom, sm.found[i]) == K - 1) sm.bound = sm.found[i];
+      __syncthreads();
+      bound = sm.bound;
+      if (tid == 0) sm.n_found = 0;
+      __syncthreads();
+    }
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long k = sm.found[i];
+      const int place = rank_of(sm.found, n, k);
+      if (place < K) sm.best[rank][place] = k;
     }
     __syncthreads();
   }
 
   // ---- sums of the CTA, then of the cluster ----------------------------------------------------------------------------------------------------
+  auto over_warp = [&](auto a) {
 #pragma unroll
-  for (int x = 16; x; x >>= 1) {
-    Sums b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, x);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, x);
-    b.t = __shfl_xor_sync(0xffffffffu, a.t, x);
-    a = join(a, b);
-  }
-  if (lane == 0) sm.warp[warp] = a;
+    for (int x = 16; x; x >>= 1) {
+      auto b = a;
+      b.m = __shfl_xor_sync(0xffffffffu, a.m, x);
+      b.s = __shfl_xor_sync(0xffffffffu, a.s, x);
+      b.t = __shfl_xor_sync(0xffffffffu, a.t, x);
+      a = join(a, b);
+    }
+    return a;
+  };
+  a = over_warp(a);
+  if (lane == 0) sm.fast[warp] = a;
   __syncthreads();
+  if (warp == 0) {  // WARPS numbers, over the lanes again
+    a = over_warp(lane < WARPS ? sm.fast[lane] : fast_nothing());
+    if (lane == 0) sm.warp[0] = natural(a);
+  }
   if (cluster > 1) {
     ptx::cluster_wait();
     if (tid == 0) {
-      a = sm.warp[0];
-      for (int w = 1; w < WARPS; ++w) a = join(a, sm.warp[w]);
+      const Sums mine = sm.warp[0];
       const uint32_t dst = ptx::mapa(ptx::smem_u32(&sm.rank[rank]), 0);
-      ptx::st_cluster_f32(dst, a.m);
-      ptx::st_cluster_f32(dst + 4, a.s);
-      ptx::st_cluster_f32(dst + 8, a.t);
+      ptx::st_cluster_f32(dst, mine.m);
+      ptx::st_cluster_f32(dst + 4, mine.s);
+      ptx::st_cluster_f32(dst + 8, mine.t);
     }
     if (TOP && rank > 0 && tid < kMaxTopLogprobs) {
       const unsigned long long k = sm.best[rank][tid];
@@ -351,18 +432,35 @@ __global__ void __launch_bounds__(WARPS * 32) token_logprobs_kernel(const Logpro
     ptx::cluster_wait();
     if (rank != 0) return;
   }
+  Sums sum = nothing();
   if (tid == 0) {
-    a = cluster > 1 ? sm.rank[0] : sm.warp[0];
-    const int n = cluster > 1 ? cluster : WARPS;
-    for (int w = 1; w < n; ++w) a = join(a, cluster > 1 ? sm.rank[w] : sm.warp[w]);
+    sum = cluster > 1 ? sm.rank[0] : sm.warp[0];
+    for (int w = 1; w < cluster; ++w) sum = join(sum, sm.rank[w]);
+    sm.special = !(sum.s > 0.f && sum.s < INFINITY && fabsf(sum.t) < INFINITY && sum.m > Vec<T>::kLow);
+  }
+  __syncthreads();
+  if (sm.special) {  // the whole row once more, value by value
+    sum = nothing();
+    for (int i = tid; i < p.vocab; i += kThreads) {
+      const float x = Vec<T>::one(row + i);
+      if (!(x - sum.m <= kLag)) rebase(sum, x);
+      add(sum, x);
+    }
+    sum = over_warp(sum);
+    if (lane == 0) sm.warp[warp] = sum;
+    __syncthreads();
+    if (tid == 0)
+      for (int w = 1; w < WARPS; ++w) sum = join(sum, sm.warp[w]);
+  }
+  if (tid == 0) {
     const long long target = p.targets[r], at = target - p.vocab_base;
     const bool here = target >= 0 && at >= 0 && at < p.vocab;
     const float xt = here ? Vec<T>::one(row + at) : __uint_as_float(kAbsent);
     if (p.partial) {
       float* out = p.partial + (size_t)r * (4 + 2 * p.top);
-      out[0] = a.m, out[1] = a.s, out[2] = a.t, out[3] = xt;
+      out[0] = sum.m, out[1] = sum.s, out[2] = sum.t, out[3] = xt;
     } else {
-      const RowResult f = finish(a, target, p.vocab_total, xt);
+      const RowResult f = finish(sum, target, p.vocab_total, xt);
       p.lse[r] = f.lse;
       p.logprob[r] = f.logprob;
       p.entropy[r] = f.entropy;
@@ -372,18 +470,19 @@ __global__ void __launch_bounds__(WARPS * 32) token_logprobs_kernel(const Logpro
   if constexpr (TOP) {
     __syncthreads();
     const int K = p.top;
-    for (int i = tid; i < cluster * 32; i += kThreads) {
-      const int c = i >> 5;
-      const unsigned long long k = sm.best[c][i & 31];
-      if ((i & 31) >= K) continue;
-      int place = i & 31;
-      if (k != 0)
-        for (int w = 0; w < cluster; ++w) {
-          if (w == c) continue;
-          for (int e = 0; e < K && sm.best[w][e] > k; ++e) ++place;
-        }
-      else if (cluster > 1)
-        continue;  // (there are K real ones: the vocabulary has at least K ids, and a shard is checked below)
+    for (int i = tid; i < cluster * K; i += kThreads) {
+      const int c = i / K, e = i - c * K;
+      const unsigned long long k = sm.best[c][e];
+      if (k == 0 && cluster > 1) continue;  // (a row that is split has K real ones; a shard with fewer columns than K is not split)
+      int place = e;                        // better ones of its own CTA, and of the others, which are in order too
+#pragma unroll 4
+      for (int w = 0; w < cluster; ++w) {
+        int at = 0;
+#pragma unroll
+        for (int step = kMaxTopLogprobs / 2; step; step >>= 1) at += sm.best[w][at + step - 1] > k ? step : 0;
+        at += sm.best[w][at] > k;
+        place += w == c ? 0 : at;
+      }
       if (place >= K) continue;
       if (p.partial) {
         float* out = p.partial + (size_t)r * (4 + 2 * K) + 4;
@@ -552,12 +651,12 @@ cudaError_t launch_forward(const LogprobParams& p, int cluster, cudaStream_t str
 
 template <typename T>
 cudaError_t forward(const LogprobParams& p, cudaStream_t stream) {
-  // a cluster for a row while the CTAs (two of 512 threads on an SM) do not fill the GPU and each still has a vector for every thread
   const long long vecs = p.vocab / Vec<T>::N;
   if (vecs <= 512) return launch_forward<T, 4>(p, 1, stream);
+  // a cluster for a row while the CTAs (six of 256 threads on an SM) do not fill the GPU and each still has four vectors for every thread
   int cluster = 1;
-  while (cluster < kMaxCluster && (long long)p.rows * cluster * 2 <= 2 * 148 && vecs >= 512ll * cluster * 2) cluster *= 2;
-  return launch_forward<T, 16>(p, cluster, stream);
+  while (cluster < kMaxCluster && (long long)p.rows * cluster * 2 <= 4 * 148 && vecs >= kClusterVecs * cluster * 2) cluster *= 2;
+  return launch_forward<T, 8>(p, cluster, stream);
 }
 
 template <typename T>

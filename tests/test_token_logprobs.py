@@ -286,3 +286,11 @@ def test_group_of_one_rank():
         assert ((da.double() - db.double()).abs() <= db.double().abs() * 2.0**-7 + 2.0**-18).all()
     finally:
         dist.destroy_process_group()
+
+
+def test_second_derivatives_are_refused():
+    x, t = inputs(3, 40, F32)
+    x.requires_grad_(True)
+    d, = torch.autograd.grad(ops.token_logprobs(x, t).entropy.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.square().sum(), x)

@@ -16,9 +16,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def _forward(logits, targets, top, group):
-    """({logprob, entropy, lse, top_logprobs, top_ids}, first column's id, vocabulary)"""
-    if group is None:
-        return _ops.token_logprobs.default(logits, targets, top), 0, logits.shape[-1]
+    """({logprob, entropy, lse, top_logprobs, top_ids}, first column's id, vocabulary) of the shards of a group"""
     world, rank = dist.get_world_size(group), dist.get_rank(group)
     base, total = rank * logits.shape[-1], world * logits.shape[-1]
     mine = _ops.token_logprobs_shard.default(logits, targets, top, base, total)
@@ -28,7 +26,9 @@ def _forward(logits, targets, top, group):
     return _ops.token_logprobs_merge.default(every, targets, top, total), base, total
 
 
-class _TokenLogprobs(torch.autograd.Function):
+class _ShardLogprobs(torch.autograd.Function):
+    """Of a rank's shard; the whole vocabulary's gradient is registered with the op."""
+
     @staticmethod
     def forward(ctx, logits, targets, top, group):
         (logprob, entropy, lse, top_logprobs, top_ids), ctx.base, ctx.total = _forward(logits, targets, top, group)
@@ -56,8 +56,10 @@ def token_logprobs(logits, targets, top=0, group=None):
 
     group: `logits` are this rank's equal shard of the vocabulary (rank 0 has the first ids); every rank passes the same targets, gets
     the whole vocabulary's results, and the gradient of its own shard. None: `logits` have the whole vocabulary."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        logprob, entropy, top_logprobs, top_ids = _TokenLogprobs.apply(logits, targets, top, group)
+    if group is None:
+        logprob, entropy, _, top_logprobs, top_ids = _ops.token_logprobs.default(logits, targets, top)
+    elif torch.is_grad_enabled() and logits.requires_grad:
+        logprob, entropy, top_logprobs, top_ids = _ShardLogprobs.apply(logits, targets, top, group)
     else:
         (logprob, entropy, _, top_logprobs, top_ids), _, _ = _forward(logits, targets, top, group)
     return TokenLogprobs(logprob, entropy, top_logprobs, top_ids) if top else TokenLogprobs(logprob, entropy, None, None)
