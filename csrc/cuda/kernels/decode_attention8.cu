@@ -230,7 +230,8 @@ __device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b
   const float scale_k = scale_of<INT8>(bits_f(seen_k)), scale_v = scale_of<INT8>(bits_f(seen_v));
   uint2* to_k = reinterpret_cast<uint2*>(c.k + sc * c.block * D);
   uint2* to_v = reinterpret_cast<uint2*>(c.v + sc * c.block * D);
-  auto codes8 = [](const uint4& w, float scale) {
+  const Divisor by_k = divisor(scale_k), by_v = divisor(scale_v);
+  auto codes8 = [](const uint4& w, const Divisor& scale) {
     return make_uint2(codes4<INT8>(lo_f(w.x), hi_f(w.x), lo_f(w.y), hi_f(w.y), scale), codes4<INT8>(lo_f(w.z), hi_f(w.z), lo_f(w.w), hi_f(w.w), scale));
   };
   for (int i0 = tid; i0 < n; i0 += U * kThreads) {
@@ -239,8 +240,8 @@ __device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * kThreads;
       if (i < n) {
-        to_k[i] = codes8(x[u], scale_k);
-        to_v[i] = codes8(y[u], scale_v);
+        to_k[i] = codes8(x[u], by_k);
+        to_v[i] = codes8(y[u], by_v);
       }
     }
   }

@@ -1,7 +1,7 @@
 // Rotary embedding of prompt rows and their quantisation into the 8-bit cache's pages, one pass over the QKV projection.
 //
 // Bound by memory: q, k and v are read once, q and k written back rotated (bf16, for the prompt's own attention), k and v written as one
-// byte each. A CTA takes `block` rows of the projection and a few heads of one kind (q, k or v). For k and v its unit is a cache block:
+// byte each (16 x 1024 rows of 32 + 32 + 32 heads: 167 us, 4.9 TB/s). A CTA takes `block` rows of the projection and a few heads of one kind (q, k or v). For k and v its unit is a cache block:
 // one thread per 16 values (8 dims and the 8 that the rotation pairs them with) of a position, so that a whole block is in the registers
 // of the CTA when its largest magnitude is known, and is read once. Rotary tables are loaded once for all heads of the CTA.
 //
@@ -46,9 +46,9 @@ __device__ __forceinline__ Unit unit_at(const KvAppend8Params& p, int row) {
   return u;
 }
 
-// D / 16 threads share a position: thread `j` has dims 8j .. 8j + 7 and those D / 2 further on.
+// D / 16 threads share a position: thread `j` has dims 8j .. 8j + 7 and those D / 2 further on. `there`: lo and hi hold them already.
 template <int D, bool INT8, bool IS_K, int HEADS>
-__device__ __forceinline__ void do_unit(const KvAppend8Params& p, const Unit& u, int kvh0, uint32_t (*s_amax)[32]) {
+__device__ __forceinline__ void do_unit(const KvAppend8Params& p, const Unit& u, int kvh0, uint32_t (*s_amax)[32], bool there, uint4 (&lo)[HEADS], uint4 (&hi)[HEADS]) {
   constexpr int J = D / 16;
   const KvCache8& c = p.cache;
   const int tid = threadIdx.x, place = tid / J, j = tid - place * J;
@@ -57,17 +57,18 @@ __device__ __forceinline__ void do_unit(const KvAppend8Params& p, const Unit& u,
   const bool fresh = place >= u.place && place < end;
   const bool old = full && place < u.place;
   const size_t row = (size_t)u.row + place - u.place;
-  uint4 lo[HEADS], hi[HEADS];
   __nv_bfloat16* tail0 = (IS_K ? c.k_tail : c.v_tail) + (((size_t)u.request * c.n_kv_heads + kvh0) * c.block + place) * D + j * 8;
   const size_t tail_step = (size_t)c.block * D;
   const __nv_bfloat16* src = p.qkv + row * p.qkv_stride + (size_t)(p.n_heads + (IS_K ? 0 : c.n_kv_heads) + kvh0) * D + j * 8;
+  if (!there) {
 #pragma unroll
-  for (int h = 0; h < HEADS; ++h) {
-    lo[h] = hi[h] = make_uint4(0, 0, 0, 0);
-    if ((fresh || old) && kvh0 + h < c.n_kv_heads) {
-      const __nv_bfloat16* at = fresh ? src + h * D : tail0 + h * tail_step;
-      lo[h] = *reinterpret_cast<const uint4*>(at);
-      hi[h] = *reinterpret_cast<const uint4*>(at + D / 2);
+    for (int h = 0; h < HEADS; ++h) {
+      lo[h] = hi[h] = make_uint4(0, 0, 0, 0);
+      if ((fresh || old) && kvh0 + h < c.n_kv_heads) {
+        const __nv_bfloat16* at = fresh ? src + h * D : tail0 + h * tail_step;
+        lo[h] = *reinterpret_cast<const uint4*>(at);
+        hi[h] = *reinterpret_cast<const uint4*>(at + D / 2);
+      }
     }
   }
   if (IS_K && fresh) {
@@ -125,8 +126,9 @@ __device__ __forceinline__ void do_unit(const KvAppend8Params& p, const Unit& u,
     const size_t sc = (size_t)u.page * c.n_kv_heads + kvh0 + h;
     uint8_t* dst = (IS_K ? c.k : c.v) + (sc * c.block + place) * D + j * 8;
     const uint4 x = lo[h], y = hi[h];
-    *reinterpret_cast<uint2*>(dst) = make_uint2(codes4<INT8>(lo_f(x.x), hi_f(x.x), lo_f(x.y), hi_f(x.y), scale), codes4<INT8>(lo_f(x.z), hi_f(x.z), lo_f(x.w), hi_f(x.w), scale));
-    *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(codes4<INT8>(lo_f(y.x), hi_f(y.x), lo_f(y.y), hi_f(y.y), scale), codes4<INT8>(lo_f(y.z), hi_f(y.z), lo_f(y.w), hi_f(y.w), scale));
+    const Divisor by = divisor(scale);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(codes4<INT8>(lo_f(x.x), hi_f(x.x), lo_f(x.y), hi_f(x.y), by), codes4<INT8>(lo_f(x.z), hi_f(x.z), lo_f(x.w), hi_f(x.w), by));
+    *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(codes4<INT8>(lo_f(y.x), hi_f(y.x), lo_f(y.y), hi_f(y.y), by), codes4<INT8>(lo_f(y.z), hi_f(y.z), lo_f(y.w), hi_f(y.w), by));
     if (tid == 0) (IS_K ? c.k_scale : c.v_scale)[sc] = scale;
   }
   __syncthreads();  // s_amax is free again; what this unit read of the tail is read
@@ -134,7 +136,23 @@ __device__ __forceinline__ void do_unit(const KvAppend8Params& p, const Unit& u,
 
 template <int D, bool INT8, bool IS_K, int HEADS>
 __device__ __forceinline__ void do_cache(const KvAppend8Params& p, int row0, int kvh0, uint32_t* s_starts, uint32_t (*s_amax)[32]) {
+  constexpr int J = D / 16;
   const int tid = threadIdx.x, block = p.cache.block;
+  // The usual unit starts with the CTA's first row and is as long: its values are asked for before that is known (three loads, one after the
+  // other, would come first).
+  uint4 lo[HEADS], hi[HEADS];
+  {
+    const size_t row = (size_t)row0 + tid / J;
+    const __nv_bfloat16* src = p.qkv + row * p.qkv_stride + (size_t)(p.n_heads + (IS_K ? 0 : p.cache.n_kv_heads) + kvh0) * D + tid % J * 8;
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      lo[h] = hi[h] = make_uint4(0, 0, 0, 0);
+      if (row < (size_t)p.rows && kvh0 + h < p.cache.n_kv_heads) {
+        lo[h] = ptx::ld_nc_v4(src + h * D);
+        hi[h] = ptx::ld_nc_v4(src + h * D + D / 2);
+      }
+    }
+  }
   // which rows start a unit: a bit for each (block <= 128 rows; a row is looked at by one thread)
   if (tid < 4) s_starts[tid] = 0;
   __syncthreads();
@@ -158,13 +176,13 @@ __device__ __forceinline__ void do_cache(const KvAppend8Params& p, int row0, int
       const int place0 = p.positions[first] & (block - 1);
       const bool ends = u.place + u.n < block;                    // it does not fill its block: it goes to the tail
       if (ends && row != first && place0 != 0) continue;          // ... which the CTA of the first unit does
-      do_unit<D, INT8, IS_K, HEADS>(p, u, kvh0, s_amax);
+      do_unit<D, INT8, IS_K, HEADS>(p, u, kvh0, s_amax, row == row0 && u.n == block, lo, hi);
       if (row == first && place0 != 0 && !ends) {
         const int last = min(p.starts[u.request + 1], p.rows) - 1;
         const int tail_row = last - (p.positions[last] & (block - 1));  // where the last block starts
         if (last > row && tail_row >= row + u.n && row_ok(p, tail_row) && p.requests[tail_row] == u.request) {
           const Unit e = unit_at(p, tail_row);
-          if (e.place == 0 && e.n < block) do_unit<D, INT8, IS_K, HEADS>(p, e, kvh0, s_amax);
+          if (e.place == 0 && e.n < block) do_unit<D, INT8, IS_K, HEADS>(p, e, kvh0, s_amax, false, lo, hi);
         }
       }
     }
@@ -218,9 +236,9 @@ __device__ __forceinline__ void do_q(const KvAppend8Params& p, int row0, int h0)
   }
 }
 
-// blockIdx.x: rows; blockIdx.y: groups of k heads, then of v heads, then of q heads.
-template <int D, bool INT8, int HEADS>
-__global__ void __launch_bounds__(1024) kv_append8_kernel(const KvAppend8Params p) {
+// blockIdx.x: rows; blockIdx.y: groups of HEADS k heads, then of v heads, then of QHEADS q heads.
+template <int D, bool INT8, int HEADS, int QHEADS, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) kv_append8_kernel(const KvAppend8Params p) {
   __shared__ uint32_t s_starts[4];
   __shared__ uint32_t s_amax[HEADS][32];
   // no early start for the kernel behind it: a GEMM fetches what it takes for weights before it waits, and this kernel's results may be that
@@ -233,13 +251,12 @@ __global__ void __launch_bounds__(1024) kv_append8_kernel(const KvAppend8Params 
   else if (y < 2 * kv_groups)
     do_cache<D, INT8, false, HEADS>(p, row0, (y - kv_groups) * HEADS, s_starts, s_amax);
   else
-    do_q<D, HEADS>(p, row0, (y - 2 * kv_groups) * HEADS);
+    do_q<D, QHEADS>(p, row0, (y - 2 * kv_groups) * QHEADS);
 }
 
-template <int D, bool INT8>
+template <int D, bool INT8, int HEADS, int QHEADS, int THREADS, int CTAS>
 cudaError_t launch(const KvAppend8Params& p, cudaStream_t stream) {
-  constexpr int HEADS = 2;
-  const int kv_groups = (p.cache.n_kv_heads + HEADS - 1) / HEADS, q_groups = (p.n_heads + HEADS - 1) / HEADS;
+  const int kv_groups = (p.cache.n_kv_heads + HEADS - 1) / HEADS, q_groups = (p.n_heads + QHEADS - 1) / QHEADS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.rows + p.cache.block - 1) / p.cache.block), 2 * kv_groups + q_groups);
   cfg.blockDim = dim3(p.cache.block * (D / 16));
@@ -247,9 +264,18 @@ cudaError_t launch(const KvAppend8Params& p, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
   cfg.attrs = attr;
   cfg.numAttrs = pdl_launch_attr(&attr[0]);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kv_append8_kernel<D, INT8, HEADS>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv_append8_kernel<D, INT8, HEADS, QHEADS, THREADS, CTAS>, p);
   if (e == cudaSuccess) launch_count_add(1);
   return e;
+}
+template <int D, bool INT8>
+cudaError_t by_size(const KvAppend8Params& p, cudaStream_t s) {
+  // Two heads of the cache and four of q a CTA, at 64 registers (us at 16 x 1024 rows of 32 + 32 + 32 heads in blocks of 32: two and two
+  // heads 170, four and four 181, one and one 200; of 16: 163, of 64: 180, of 128: 203).
+  const int threads = p.cache.block * (D / 16);
+  if (threads <= 256) return launch<D, INT8, 2, 4, 256, 4>(p, s);
+  if (threads <= 512) return launch<D, INT8, 2, 4, 512, 2>(p, s);
+  return launch<D, INT8, 2, 4, 1024, 1>(p, s);
 }
 
 }  // namespace
@@ -263,8 +289,8 @@ cudaError_t kv_append8(const KvAppend8Params& p, cudaStream_t stream) {
   if (2ll * c.n_kv_heads + p.n_heads > 65535) return cudaErrorInvalidValue;
   if (!aligned(p.qkv) || !aligned(p.rotated) || !aligned(c.k) || !aligned(c.v) || !aligned(c.k_tail) || !aligned(c.v_tail) || !aligned(p.cos) || !aligned(p.sin)) return cudaErrorInvalidValue;
   if (p.qkv_stride % 8 != 0 || p.rotated_stride % 8 != 0) return cudaErrorInvalidValue;
-  if (c.head_dim == 128) return c.int8 ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
-  if (c.head_dim == 64) return c.int8 ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
+  if (c.head_dim == 128) return c.int8 ? by_size<128, true>(p, stream) : by_size<128, false>(p, stream);
+  if (c.head_dim == 64) return c.int8 ? by_size<64, true>(p, stream) : by_size<64, false>(p, stream);
   return cudaErrorInvalidValue;
 }
 

@@ -26,13 +26,24 @@ __device__ __forceinline__ float scale_of(float amax) {
   const float s = __fdiv_rn(amax, INT8 ? 127.f : 448.f);
   return s < kLeastScale ? kLeastScale : s;  // (a NaN stays)
 }
+// A scale that many values are divided by. With the correctly rounded reciprocal r, q = x r is corrected by its residual to the correctly
+// rounded quotient, q + (x - q s) r (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990):
+// three operations a value where a division is a dozen. (A quotient so small that the residual is not exact has the code zero anyhow.)
+struct Divisor {
+  float s, r;  // r 0: s is not finite, and is divided by
+};
+__device__ __forceinline__ Divisor divisor(float s) { return {s, s < INFINITY ? __frcp_rn(s) : 0.f}; }
+__device__ __forceinline__ float over(float x, const Divisor& d) {
+  const float q = x * d.r;
+  return d.r == 0.f ? __fdiv_rn(x, d.s) : fmaf(fmaf(-q, d.s, x), d.r, q);
+}
 // Four values over one scale -> four codes.
 template <bool INT8>
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float scale) {
-  a = __fdiv_rn(a, scale);
-  b = __fdiv_rn(b, scale);
-  c = __fdiv_rn(c, scale);
-  d = __fdiv_rn(d, scale);
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, const Divisor& scale) {
+  a = over(a, scale);
+  b = over(b, scale);
+  c = over(c, scale);
+  d = over(d, scale);
   if constexpr (INT8) {
     auto q = [](float x) { return (uint32_t)(max(-127, min(127, __float2int_rn(x))) & 0xff); };
     return q(a) | (q(b) << 8) | (q(c) << 16) | (q(d) << 24);
