@@ -10,6 +10,10 @@ Every hot op of a decode step is a kernel of this repository:
     and the following RMSNorm (the pattern the reference's LLM all-reduce path targets,
     tests/test_allreduce.py:51-67 and src/gpu/allreduce_small.h of intel/torch-ccl).
 
+With kv_cache="fp8" or "int8" the KV cache is held in 8 bits, in pages of one pool that every step takes what it needs from (ops.kv_plan,
+ops.decode_attention_8bit); with logprobs=n every step also leaves the log-probabilities of the sampled ids, the entropies and the n best
+alternatives (ops.token_logprobs), and `score` gives them for the ids of a prompt.
+
 The whole step is captured in one CUDA graph. Weights are random N(0, 0.02) in bf16, generated
 from per-matrix seeds so that every tensor-parallel degree shards the same full model.
 """
@@ -20,7 +24,8 @@ import torch
 import torch.distributed as dist
 
 from .. import _C
-from ..ops import pack_weight, unpack_weight
+from ..ops import (KVBlocks, KVCache8, TokenLogprobs, decode_attention_8bit, kv_append_8bit, kv_plan, kv_release, pack_weight, token_logprobs,
+                   unpack_weight)
 
 
 @dataclass
@@ -133,12 +138,17 @@ class TPLlamaDecoder:
     """Llama decoder sharded `world`-way by attention head and FFN column (Megatron layout)."""
 
     def __init__(self, cfg: LlamaConfig, max_batch=16, max_seq=2048, group=None, device=None, seed=0, collective="ccl",
-                 fused=True):
+                 fused=True, kv_cache="bf16", kv_block=32, kv_blocks=None, logprobs=None):
         """fused=True (default): 5 kernels per layer - qkv GEMM, attention, o_proj GEMM + all_reduce +
         residual + norm in one launch, gate/up GEMM + SwiGLU, down_proj GEMM + all_reduce + residual +
         norm in one launch - plus embedding + first norm, lm_head and the sampling kernel per step.
         fused=False: the projections, the all_reduce + norm and the sampling run as separate kernels
-        (7 per layer); kept for A/B measurements. collective="nccl" implies fused=False."""
+        (7 per layer); kept for A/B measurements. collective="nccl" implies fused=False.
+
+        kv_cache: "bf16" (dense, max_seq positions a sequence), or "fp8" / "int8": pages of kv_block positions (16, 32, 64 or 128) with one
+        scale each, kv_blocks of them for all sequences (default: as many as max_batch sequences of max_seq need). A step that the
+        pool has too few pages for leaves `blocks.state[1]` (sequences not served) above zero; such a sequence's results are void.
+        logprobs: None, or how many alternatives (0 to 32) `last_logprobs` gives beside the log-probability of every sampled id."""
         self.cfg = cfg
         self.device = torch.device(device if device is not None else f"cuda:{torch.cuda.current_device()}")
         self.comm = _Comm(group, self.device, collective)
@@ -147,6 +157,10 @@ class TPLlamaDecoder:
         self.world, self.rank = W, r
         assert cfg.n_heads % W == 0 and cfg.n_kv_heads % W == 0 and cfg.inter % (8 * W) == 0 and cfg.vocab % W == 0
         assert cfg.head_dim == 128, "decode attention kernel is specialised for head_dim 128"
+        assert kv_cache in ("bf16", "fp8", "int8"), "kv_cache: bf16, fp8 or int8"
+        assert logprobs is None or (0 <= logprobs <= 32 and collective == "ccl"), "logprobs: None or 0 to 32, on the ccl backend"
+        self.kv_cache, self.kv_block, self.logprobs = kv_cache, kv_block, logprobs
+        self.group = (group if group is not None else dist.group.WORLD) if W > 1 else None
         self.max_batch, self.max_seq = max_batch, max_seq
         self.nh = cfg.n_heads // W
         self.nkv = cfg.n_kv_heads // W
@@ -155,6 +169,11 @@ class TPLlamaDecoder:
         hd, H = cfg.head_dim, cfg.hidden
         dev = self.device
         self.layers = []
+        self.blocks = None
+        if kv_cache != "bf16":
+            per_seq = (max_seq + kv_block - 1) // kv_block
+            kv_blocks = kv_blocks if kv_blocks is not None else max_batch * per_seq
+            self.blocks = KVBlocks.empty(max_batch, per_seq, kv_blocks, dev)
         for li in range(cfg.n_layers):
             s = seed * 100003 + li * 16
             wq = _rand((cfg.n_heads * hd, H), s + 1, dev)[r * self.nh * hd:(r + 1) * self.nh * hd]
@@ -170,9 +189,13 @@ class TPLlamaDecoder:
                 wqkv=pack_weight(torch.cat([wq, wk, wv])), wo=pack_weight(wo),
                 wgu=torch.cat([pack_weight(wg), pack_weight(wu)]), wd=pack_weight(wd),
                 attn_norm=torch.ones(H, device=dev, dtype=torch.bfloat16),
-                mlp_norm=torch.ones(H, device=dev, dtype=torch.bfloat16),
-                k=torch.zeros(max_batch, self.nkv, max_seq, hd, device=dev, dtype=torch.bfloat16),
-                v=torch.zeros(max_batch, self.nkv, max_seq, hd, device=dev, dtype=torch.bfloat16)))
+                mlp_norm=torch.ones(H, device=dev, dtype=torch.bfloat16)))
+            if self.blocks is None:
+                self.layers[-1].update(k=torch.zeros(max_batch, self.nkv, max_seq, hd, device=dev, dtype=torch.bfloat16),
+                                       v=torch.zeros(max_batch, self.nkv, max_seq, hd, device=dev, dtype=torch.bfloat16))
+            else:
+                self.layers[-1]["cache"] = KVCache8.empty(kv_blocks, self.nkv, kv_block, hd, max_batch,
+                                                          torch.float8_e4m3fn if kv_cache == "fp8" else torch.int8, dev)
             del wq, wk, wv, wo, wg, wu, wd
         self.embed = _rand((cfg.vocab, H), seed * 100003 + 900001, dev)[r * self.vshard:(r + 1) * self.vshard].contiguous()
         self.lm_head = pack_weight(_rand((cfg.vocab, H), seed * 100003 + 900002, dev)[r * self.vshard:(r + 1) * self.vshard])
@@ -204,6 +227,9 @@ class TPLlamaDecoder:
         self.graph_batch = None
         # (the unfused path also runs ~20 small torch kernels per step that are not counted here)
         self.kernels_per_step = cfg.n_layers * 5 + 3 if self.fused else cfg.n_layers * 7 + 2 + (1 if W > 1 else 0)
+        self.kernels_per_step += (1 if self.blocks is not None else 0) + (0 if logprobs is None else 1 if W == 1 else 3)
+        self.last_logprobs = None  # of the last step's ids: a TokenLogprobs
+        self.graph_logprobs = None
         self._pin_in = None
         self._pin_out = None
 
@@ -241,21 +267,48 @@ class TPLlamaDecoder:
     def _next_norm(self, li):
         return self.layers[li + 1]["attn_norm"] if li + 1 < self.cfg.n_layers else self.final_norm
 
-    def _layer_fused(self, li, B, k, v, positions):
+    def _attend(self, L, B, positions):
+        """Rotary embedding, append and attention of one new token for each of B sequences: qkv -> attn."""
+        qkv, attn = self.qkv[:B], self.attn[:B]
+        if self.blocks is not None:
+            decode_attention_8bit(qkv, positions, self.blocks.table, L["cache"], self.cos, self.sin, self.nh, out=attn)
+        else:
+            _C.decode_attention(qkv, L["k"], L["v"], positions, self.cos, self.sin, attn, self.scratch, self.counters, self.nh, self.nkv, self.nsplit)
+
+    def _take_pages(self, B):
+        """Pages for one more position of each of B sequences (none for rows whose position is negative)."""
+        if self.blocks is not None:
+            kv_plan(self.positions[:B], None, self.blocks.rows(0, B), self.kv_block)
+
+    def _leave_logprobs(self, B):
+        if self.logprobs is not None:
+            self.last_logprobs = token_logprobs(self.logits[:B], self.next_tokens[:B], self.logprobs, self.group)
+
+    def finish(self, rows):
+        """Ends the sequences in these rows of the batch: their pages (8-bit cache) go back to the pool and the rows are idle, at position -1 and
+        below, until the next prefill."""
+        done = torch.zeros(self.max_batch, dtype=torch.bool)
+        done[list(rows)] = True
+        done = done.to(self.device)
+        if self.blocks is not None:
+            kv_release(done, self.blocks)
+        self.positions.masked_fill_(done, -(1 << 30))
+
+    def _layer_fused(self, li, B, positions):
         """One layer for one new token of each of B sequences: xn is normalised again for the next layer."""
         L, cfg = self.layers[li], self.cfg
         h, xn, qkv, attn, act = self.h[:B], self.xn[:B], self.qkv[:B], self.attn[:B], self.act[:B]
         self._gemm_t(L["wqkv"], xn, qkv, self.qkv_rows)
-        _C.decode_attention(qkv, k, v, positions, self.cos, self.sin, attn, self.scratch, self.counters, self.nh, self.nkv, self.nsplit)
+        self._attend(L, B, positions)
         self.comm.gemm_ar_norm(L["wo"], attn, h, L["mlp_norm"], xn, cfg.eps)
         self._gemm_t(L["wgu"], xn, act, self.inter, dual=self.inter_pad)
         self.comm.gemm_ar_norm(L["wd"], act, h, self._next_norm(li), xn, cfg.eps)
 
-    def _layer_unfused(self, li, B, k, v, positions):
+    def _layer_unfused(self, li, B, positions):
         L, cfg = self.layers[li], self.cfg
         h, x, xn, qkv, attn, act = self.h[:B], self.x[:B], self.xn[:B], self.qkv[:B], self.attn[:B], self.act[:B]
         self._gemm_t(L["wqkv"], xn, qkv, self.qkv_rows)
-        _C.decode_attention(qkv, k, v, positions, self.cos, self.sin, attn, self.scratch, self.counters, self.nh, self.nkv, self.nsplit)
+        self._attend(L, B, positions)
         self._gemm_t(L["wo"], attn, x, cfg.hidden)
         self.comm.ar_res_norm(x, h, L["mlp_norm"], xn, cfg.eps)
         self._gemm_t(L["wgu"], xn, act, self.inter, dual=self.inter_pad)
@@ -268,12 +321,14 @@ class TPLlamaDecoder:
         self.comm.embed_norm(tokens, self.embed, self.rank * self.vshard, h, self.layers[0]["attn_norm"], xn, cfg.eps)
         fused_rows = self._fused_rows(B)
         layer = self._layer_fused if fused_rows else self._layer_unfused
-        for li, L in enumerate(self.layers):
-            layer(li, B, L["k"], L["v"], self.positions[:B])
+        self._take_pages(B)
+        for li in range(cfg.n_layers):
+            layer(li, B, self.positions[:B])
         self._gemm_t(self.lm_head, xn, self.logits[:B], self.vshard)
         # feeds the sampled ids back into self.tokens and advances the positions: steady state is a pure replay
         # (batches above the fused rows choose among NaNs as torch.max does, like the unfused step)
         self.comm.sample(self.logits[:B], self.next_tokens[:B], tokens, self.positions[:B], nan_first=not fused_rows)
+        self._leave_logprobs(B)
 
     def _decode_body_unfused(self, B):
         cfg = self.cfg
@@ -281,8 +336,9 @@ class TPLlamaDecoder:
         self._embed_partial(tokens, x)
         h.zero_()
         self.comm.ar_res_norm(x, h, self.layers[0]["attn_norm"], xn, cfg.eps)
-        for li, L in enumerate(self.layers):
-            self._layer_unfused(li, B, L["k"], L["v"], self.positions[:B])
+        self._take_pages(B)
+        for li in range(cfg.n_layers):
+            self._layer_unfused(li, B, self.positions[:B])
         self._gemm_t(self.lm_head, xn, self.logits[:B], self.vshard)
         val, idx = self.logits[:B].max(dim=-1)
         if self.world > 1:
@@ -295,6 +351,7 @@ class TPLlamaDecoder:
             self.next_tokens[:B] = idx
         self.positions[:B] += 1
         self.tokens[:B] = self.next_tokens[:B]  # feed the sampled ids back: steady state is a pure replay
+        self._leave_logprobs(B)
 
     def capture(self, B):
         """Capture one decode step for batch size B in a CUDA graph."""
@@ -303,6 +360,10 @@ class TPLlamaDecoder:
         s.wait_stream(torch.cuda.current_stream(self.device))
         saved_pos = self.positions.clone()
         saved_tok = self.tokens.clone()  # the step feeds its sampled ids back into self.tokens
+        if self.blocks is not None:
+            # the warm-up steps append nothing: a position written in the next block would take the place of one in this block's tail
+            self.positions.fill_(-(1 << 20))
+            s.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(s):
             for _ in range(2):  # warm-up outside capture (lazy inits, tensor-map cache)
                 self._decode_body(B)
@@ -313,7 +374,7 @@ class TPLlamaDecoder:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=s):
             self._decode_body(B)
-        self.graph, self.graph_batch = g, B
+        self.graph, self.graph_batch, self.graph_logprobs = g, B, self.last_logprobs
         torch.cuda.synchronize(self.device)
         return g
 
@@ -323,6 +384,7 @@ class TPLlamaDecoder:
         B = B or self.graph_batch or self.max_batch
         if self.graph is not None and self.graph_batch == B:
             self.graph.replay()
+            self.last_logprobs = self.graph_logprobs
         else:
             self._decode_body(B)
         return self.next_tokens[:B]
@@ -348,6 +410,24 @@ class TPLlamaDecoder:
         sequence is wanted: the rest of that layer runs for those rows alone, with the sums over K in the order that
         they have for all rows (no split), so that a prompt's results do not depend on the shortcut.
         `chunk_seqs` bounds the sequences per pass (default: as many as keep a pass under ~32k rows)."""
+        self._prefill(prompt, chunk_seqs, None)
+
+    def score(self, prompt, top=0, chunk_seqs=None):
+        """Prefill that also gives the log-probability of every id of the prompt [B, S] after its first, the entropies there and the `top` best
+        alternatives: a TokenLogprobs of [B, S - 1] (and [B, S - 1, top])."""
+        return self._prefill(prompt, chunk_seqs, top)
+
+    def _score_rows(self, xn, targets, top):
+        """Log-probabilities of `targets` after the final norm's rows, 2048 rows of logits at a time."""
+        pieces = []
+        for r0 in range(0, xn.shape[0], 2048):
+            rows = xn[r0:r0 + 2048]
+            logits = torch.empty(rows.shape[0], self.vshard, device=self.device, dtype=torch.float32)
+            self._gemm_t(self.lm_head, rows, logits, self.vshard)
+            pieces.append(token_logprobs(logits, targets[r0:r0 + 2048], top, self.group))
+        return [torch.cat(p) if p[0] is not None else None for p in zip(*pieces)]
+
+    def _prefill(self, prompt, chunk_seqs, score_top):
         cfg = self.cfg
         B, S = prompt.shape
         hd, H = cfg.head_dim, cfg.hidden
@@ -357,6 +437,11 @@ class TPLlamaDecoder:
         cap_rows = 1024 if self.world > 1 else 1 << 30  # rows per fused-norm launch (staging capacity)
         per = chunk_seqs or max(1, 32768 // S)
         last_li = cfg.n_layers - 1
+        assert S <= self.max_seq and B <= self.max_batch, "the prompt does not fit the cache"
+        assert score_top is None or self.comm.nccl is None, "score runs on the ccl backend"
+        scored, refused = [], []
+        if self.blocks is not None:  # what the rows held before goes back to the pool
+            kv_release(torch.ones(B, dtype=torch.bool, device=dev), self.blocks.rows(0, B))
         for b0 in range(0, B, per):
             n = min(per, B - b0)
             R = n * S
@@ -385,15 +470,24 @@ class TPLlamaDecoder:
                     self.comm.embed_norm(toks[r0:r1], self.embed, self.rank * self.vshard, h[r0:r1], self.layers[0]["attn_norm"],
                                          xn[r0:r1], cfg.eps)
             splitk = 0
+            if self.blocks is not None:
+                none, new = torch.zeros(n, dtype=torch.int32, device=dev), torch.full((n,), S, dtype=torch.int32, device=dev)
+                plan = kv_plan(none, new, self.blocks.rows(b0, b0 + n), self.kv_block, R)
+                refused.append(self.blocks.state[1].clone())
             for li, L in enumerate(self.layers):
-                k, v = L["k"][b0:b0 + n], L["v"][b0:b0 + n]
                 self._gemm_t(L["wqkv"], xn, qkv, self.qkv_rows)
-                _C.rope_append(qkv, k, v, self.cos, self.sin, self.nh, S)
-                o = torch.nn.functional.scaled_dot_product_attention(
-                    qkv.view(n, S, -1)[..., :nq].view(n, S, self.nh, hd).transpose(1, 2), k[:, :, :S], v[:, :, :S], is_causal=True,
-                    enable_gqa=self.nh != self.nkv).transpose(1, 2)
+                heads = qkv.view(n, S, -1, hd)
+                if self.blocks is not None:  # the prompt attends to its own keys and values, as bf16
+                    rotated = kv_append_8bit(qkv, plan, L["cache"].rows(b0, b0 + n), self.cos, self.sin, self.nh).view(n, S, -1, hd)
+                    q, k, v = rotated[:, :, :self.nh], rotated[:, :, self.nh:].transpose(1, 2), heads[:, :, self.nh + self.nkv:].transpose(1, 2)
+                else:
+                    k, v = L["k"][b0:b0 + n], L["v"][b0:b0 + n]
+                    _C.rope_append(qkv, k, v, self.cos, self.sin, self.nh, S)
+                    q, k, v = heads[:, :, :self.nh], k[:, :, :S], v[:, :, :S]
+                o = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k, v, is_causal=True,
+                                                                     enable_gqa=self.nh != self.nkv).transpose(1, 2)
                 # (a chunk of at most 128 rows is one tile of rows, whatever is left out of it: it stays as it is)
-                if li == last_li and R > 128:
+                if li == last_li and R > 128 and score_top is None:
                     o, h = o[:, S - 1], h.view(n, S, H)[:, S - 1].contiguous()
                     x, xn, act, splitk = x[:n], xn[:n], act[:n], 1
                 self._gemm_t(L["wo"], o.reshape(-1, nq), x, H, splitk=splitk)
@@ -401,7 +495,12 @@ class TPLlamaDecoder:
                 self._gemm_t(L["wgu"], xn, act, self.inter, dual=self.inter_pad, splitk=splitk)
                 self._gemm_t(L["wd"], act, x, H, splitk=splitk)
                 norm_step(self._next_norm(li))
-            last = xn if R > 128 else xn.view(n, S, H)[:, S - 1].contiguous()
+            last = xn if R > 128 and score_top is None else xn.view(n, S, H)[:, S - 1].contiguous()
+            if score_top is not None:
+                after = torch.full((n, S), -1, dtype=torch.int64, device=dev)
+                after[:, :-1] = toks.view(n, S)[:, 1:]
+                got = self._score_rows(xn, after.view(-1), score_top)
+                scored.append([None if t is None else t.view(n, S, *t.shape[1:])[:, :-1] for t in got])
             logits = torch.empty(n, self.vshard, device=dev, dtype=torch.float32)
             self._gemm_t(self.lm_head, last, logits, self.vshard)
             val, idx = logits.max(dim=-1)
@@ -414,8 +513,24 @@ class TPLlamaDecoder:
             self.tokens[b0:b0 + n] = idx
         self.positions[:B] = S
         torch.cuda.synchronize(dev)
+        if any(int(r) for r in refused):
+            raise RuntimeError(f"prefill: the KV pool of {self.blocks.free.numel()} pages of {self.kv_block} positions has too few for {B} prompts of {S}")
+        return TokenLogprobs(*(None if p[0] is None else torch.cat(p) for p in zip(*scored))) if scored else None
 
     # ------------------------------------------------------------------------------------
+    def _cached(self, L, b, p):
+        """K and V of sequence b's positions 0 .. p - 1 in fp32, [nkv, p, hd] each (oracle / debugging only)."""
+        if self.blocks is None:
+            return L["k"][b, :, :p].float(), L["v"][b, :, :p].float()
+        c, bs = L["cache"], self.kv_block
+        pages = self.blocks.table[b, :p // bs].long()
+
+        def of(codes, scale, tail):
+            paged = (codes.view(torch.uint8)[pages].view(codes.dtype).float() * scale[pages][..., None, None]).transpose(0, 1)
+            return torch.cat([paged.reshape(self.nkv, -1, self.cfg.head_dim), tail[b, :, :p % bs].float()], dim=1)
+
+        return of(c.k, c.k_scale, c.k_tail), of(c.v, c.v_scale, c.v_tail)
+
     def reference_decode_step(self, B):
         """Plain PyTorch fp32 restatement of one decode step on this rank's shard plus
         torch.distributed all_reduces; the oracle of the numerics tests. Does not touch the
@@ -456,8 +571,9 @@ class TPLlamaDecoder:
             outs = []
             for b in range(B):
                 p = int(pos[b])
-                kk = torch.cat([L["k"][b, :, :p].float(), k[b][:, None, :]], dim=1)  # [nkv, p+1, hd]
-                vv = torch.cat([L["v"][b, :, :p].float(), v[b][:, None, :]], dim=1)
+                kk, vv = self._cached(L, b, p)
+                kk = torch.cat([kk, k[b][:, None, :]], dim=1)  # [nkv, p+1, hd]
+                vv = torch.cat([vv, v[b][:, None, :]], dim=1)
                 rep = self.nh // self.nkv
                 kk = kk.repeat_interleave(rep, 0)
                 vv = vv.repeat_interleave(rep, 0)
