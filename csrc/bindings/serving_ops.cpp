@@ -2,6 +2,7 @@
 //
 // Each op has one function that checks its arguments and gives its results' shapes, which the CUDA and the Meta kernel share, so that
 // tracing refuses what a launch would refuse.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -22,6 +23,38 @@ using c10::optional;
 
 void ok(cudaError_t e, const char* op) { TORCH_CHECK(e == cudaSuccess, op, ": ", cudaGetErrorString(e)); }
 cudaStream_t stream() { return c10::cuda::getCurrentCUDAStream(); }
+
+// Uninitialised tensors beside `like`.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  if (like.is_cuda()) return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+  return at::empty(sizes, like.options().dtype(type));
+}
+// Several small ones, on a GPU in one allocation: each costs the host a microsecond, of nine in a call.
+template <size_t N>
+std::array<Tensor, N> fresh_together(const Tensor& like, const std::array<std::pair<at::DimVector, at::ScalarType>, N>& what) {
+  std::array<Tensor, N> out;
+  if (!like.is_cuda()) {
+    for (size_t i = 0; i < N; ++i) out[i] = fresh(what[i].first, what[i].second, like);
+    return out;
+  }
+  auto bytes_of = [](const std::pair<at::DimVector, at::ScalarType>& w) {
+    int64_t n = (int64_t)c10::elementSize(w.second);
+    for (int64_t d : w.first) n *= d;
+    return (n + 15) / 16 * 16;
+  };
+  int64_t total = 0;
+  for (const auto& w : what) total += bytes_of(w);
+  const Tensor all = at::detail::empty_cuda({total}, at::kByte, like.device(), c10::nullopt);
+  int64_t at = 0;
+  for (size_t i = 0; i < N; ++i) {
+    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(what[i].second));
+    auto* t = out[i].unsafeGetTensorImpl();
+    t->set_storage_offset(at / (int64_t)c10::elementSize(what[i].second));
+    t->set_sizes_contiguous(what[i].first);
+    at += bytes_of(what[i]);
+  }
+  return out;
+}
 
 // A tensor of this type, rank, device and layout (all dimensions dense).
 void expect(const Tensor& t, const char* op, const char* name, at::ScalarType type, int64_t dim, const Tensor& like) {
@@ -84,8 +117,8 @@ Plan plan_shapes(const Tensor& lengths, const optional<Tensor>& new_tokens, cons
   TORCH_CHECK(block == 16 || block == 32 || block == 64 || block == 128, op, ": block_size must be 16, 32, 64 or 128, not ", block);
   TORCH_CHECK(room >= 0 && room < 0x7fffffff, op, ": max_tokens must be between 0 and 2^31 - 2");
   TORCH_CHECK(free_blocks.size(0) * block <= 0x7fffffff, op, ": slots are 32-bit: ", free_blocks.size(0), " blocks of ", block, " are too many");
-  auto i32 = lengths.options();
-  return {at::empty({lengths.size(0) + 1}, i32), at::empty({room}, i32), at::empty({room}, i32), at::empty({room}, i32)};
+  auto t = fresh_together<4>(lengths, {{{{lengths.size(0) + 1}, at::kInt}, {{room}, at::kInt}, {{room}, at::kInt}, {{room}, at::kInt}}});
+  return {t[0], t[1], t[2], t[3]};
 }
 Plan kv_plan_cuda(const Tensor& lengths, const optional<Tensor>& new_tokens, Tensor& table, Tensor& held, Tensor& free_blocks, Tensor& state, int64_t block, int64_t room) {
   c10::cuda::CUDAGuard g(lengths.device());
@@ -213,13 +246,13 @@ void append(const Tensor& qkv, PLAN_ARGS, CONST_CACHE_ARGS, const Tensor& cos, c
 Tensor kv_append_8bit_cuda(const Tensor& qkv, PLAN_ARGS, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads) {
   check_append(qkv, starts, requests, positions, slots, k, v, ks, vs, kt, vt, cos, sin, n_heads, nullptr);
   c10::cuda::CUDAGuard g(qkv.device());
-  Tensor out = at::empty({qkv.size(0), (n_heads + k.size(1)) * k.size(3)}, qkv.options());
+  Tensor out = fresh({qkv.size(0), (n_heads + k.size(1)) * k.size(3)}, at::kBFloat16, qkv);
   append(qkv, starts, requests, positions, slots, k, v, ks, vs, kt, vt, cos, sin, n_heads, out, true);
   return out;
 }
 Tensor kv_append_8bit_meta(const Tensor& qkv, PLAN_ARGS, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads) {
   check_append(qkv, starts, requests, positions, slots, k, v, ks, vs, kt, vt, cos, sin, n_heads, nullptr);
-  return at::empty({qkv.size(0), (n_heads + k.size(1)) * k.size(3)}, qkv.options());
+  return fresh({qkv.size(0), (n_heads + k.size(1)) * k.size(3)}, at::kBFloat16, qkv);
 }
 void kv_append_8bit_out_cuda(const Tensor& qkv, PLAN_ARGS, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads, Tensor& out) {
   check_append(qkv, starts, requests, positions, slots, k, v, ks, vs, kt, vt, cos, sin, n_heads, &out);
@@ -274,7 +307,7 @@ void attention(const Tensor& qkv, const Tensor& positions, const Tensor& table, 
   p.partials = nullptr;
   Tensor partials;  // of this call alone: two calls, or two captured graphs, never share it
   if (const size_t n = ccl::decode_attention8_partial_floats(p)) {
-    partials = at::empty({(int64_t)n}, qkv.options().dtype(at::kFloat));
+    partials = fresh({(int64_t)n}, at::kFloat, qkv);
     p.partials = partials.data_ptr<float>();
   }
   ok(ccl::decode_attention8(p, stream()), op);
@@ -282,13 +315,13 @@ void attention(const Tensor& qkv, const Tensor& positions, const Tensor& table, 
 Tensor decode_attention_8bit_cuda(const Tensor& qkv, const Tensor& positions, const Tensor& table, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads) {
   check_attention(qkv, positions, table, k, v, ks, vs, kt, vt, cos, sin, n_heads, nullptr);
   c10::cuda::CUDAGuard g(qkv.device());
-  Tensor out = at::empty({qkv.size(0), n_heads * k.size(3)}, qkv.options());
+  Tensor out = fresh({qkv.size(0), n_heads * k.size(3)}, at::kBFloat16, qkv);
   attention(qkv, positions, table, k, v, ks, vs, kt, vt, cos, sin, n_heads, out);
   return out;
 }
 Tensor decode_attention_8bit_meta(const Tensor& qkv, const Tensor& positions, const Tensor& table, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads) {
   check_attention(qkv, positions, table, k, v, ks, vs, kt, vt, cos, sin, n_heads, nullptr);
-  return at::empty({qkv.size(0), n_heads * k.size(3)}, qkv.options());
+  return fresh({qkv.size(0), n_heads * k.size(3)}, at::kBFloat16, qkv);
 }
 void decode_attention_8bit_out_cuda(const Tensor& qkv, const Tensor& positions, const Tensor& table, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads, Tensor& out) {
   check_attention(qkv, positions, table, k, v, ks, vs, kt, vt, cos, sin, n_heads, &out);
@@ -318,9 +351,9 @@ void check_logits(const char* op, const Tensor& logits, const Tensor& targets, i
 long long row_stride(const Tensor& logits) { return logits.size(0) > 1 ? logits.stride(0) : logits.size(1); }
 
 using Logprobs = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
-Logprobs logprob_shapes(int64_t rows, int64_t top, const at::TensorOptions& like) {
-  auto f = like.dtype(at::kFloat);
-  return {at::empty({rows}, f), at::empty({rows}, f), at::empty({rows}, f), at::empty({rows, top}, f), at::empty({rows, top}, like.dtype(at::kLong))};
+Logprobs logprob_shapes(int64_t rows, int64_t top, const Tensor& like) {
+  auto t = fresh_together<5>(like, {{{{rows}, at::kFloat}, {{rows}, at::kFloat}, {{rows}, at::kFloat}, {{rows, top}, at::kFloat}, {{rows, top}, at::kLong}}});
+  return {t[0], t[1], t[2], t[3], t[4]};
 }
 ccl::LogprobParams logprob_params(const Tensor& logits, const Tensor& targets, int64_t top, int64_t base, int64_t total) {
   ccl::LogprobParams p = {};
@@ -338,7 +371,7 @@ ccl::LogprobParams logprob_params(const Tensor& logits, const Tensor& targets, i
 Logprobs token_logprobs_cuda(const Tensor& logits, const Tensor& targets, int64_t top) {
   check_logits("token_logprobs", logits, targets, top, 0, logits.dim() == 2 ? logits.size(1) : 0);
   c10::cuda::CUDAGuard g(logits.device());
-  Logprobs out = logprob_shapes(logits.size(0), top, logits.options());
+  Logprobs out = logprob_shapes(logits.size(0), top, logits);
   auto p = logprob_params(logits, targets, top, 0, logits.size(1));
   p.logprob = std::get<0>(out).data_ptr<float>();
   p.entropy = std::get<1>(out).data_ptr<float>();
@@ -350,12 +383,12 @@ Logprobs token_logprobs_cuda(const Tensor& logits, const Tensor& targets, int64_
 }
 Logprobs token_logprobs_meta(const Tensor& logits, const Tensor& targets, int64_t top) {
   check_logits("token_logprobs", logits, targets, top, 0, logits.dim() == 2 ? logits.size(1) : 0);
-  return logprob_shapes(logits.size(0), top, logits.options());
+  return logprob_shapes(logits.size(0), top, logits);
 }
 Tensor token_logprobs_shard_cuda(const Tensor& logits, const Tensor& targets, int64_t top, int64_t base, int64_t total) {
   check_logits("token_logprobs", logits, targets, top, base, total);
   c10::cuda::CUDAGuard g(logits.device());
-  Tensor out = at::empty({logits.size(0), 4 + 2 * top}, logits.options().dtype(at::kFloat));
+  Tensor out = fresh({logits.size(0), 4 + 2 * top}, at::kFloat, logits);
   auto p = logprob_params(logits, targets, top, base, total);
   p.partial = out.data_ptr<float>();
   ok(ccl::token_logprobs(p, stream()), "token_logprobs");
@@ -363,7 +396,7 @@ Tensor token_logprobs_shard_cuda(const Tensor& logits, const Tensor& targets, in
 }
 Tensor token_logprobs_shard_meta(const Tensor& logits, const Tensor& targets, int64_t top, int64_t base, int64_t total) {
   check_logits("token_logprobs", logits, targets, top, base, total);
-  return at::empty({logits.size(0), 4 + 2 * top}, logits.options().dtype(at::kFloat));
+  return fresh({logits.size(0), 4 + 2 * top}, at::kFloat, logits);
 }
 void check_merge(const Tensor& partials, const Tensor& targets, int64_t top, int64_t total) {
   const char* op = "token_logprobs_merge";
@@ -376,7 +409,7 @@ void check_merge(const Tensor& partials, const Tensor& targets, int64_t top, int
 Logprobs token_logprobs_merge_cuda(const Tensor& partials, const Tensor& targets, int64_t top, int64_t total) {
   check_merge(partials, targets, top, total);
   c10::cuda::CUDAGuard g(partials.device());
-  Logprobs out = logprob_shapes(partials.size(1), top, partials.options());
+  Logprobs out = logprob_shapes(partials.size(1), top, partials);
   ccl::LogprobMergeParams p;
   p.partials = partials.data_ptr<float>();
   p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
@@ -394,7 +427,7 @@ Logprobs token_logprobs_merge_cuda(const Tensor& partials, const Tensor& targets
 }
 Logprobs token_logprobs_merge_meta(const Tensor& partials, const Tensor& targets, int64_t top, int64_t total) {
   check_merge(partials, targets, top, total);
-  return logprob_shapes(partials.size(1), top, partials.options());
+  return logprob_shapes(partials.size(1), top, partials);
 }
 
 void check_backward(const Tensor& logits, const Tensor& targets, const Tensor& lse, const Tensor& entropy, const Tensor& top_ids, const optional<Tensor>& g_lp, const optional<Tensor>& g_ent,
@@ -420,7 +453,7 @@ Tensor token_logprobs_backward_cuda(const Tensor& logits, const Tensor& targets,
   // the gradient's rows lie as the logits' rows do relative to 16 bytes, so that one vector of the one is one of the other
   const int64_t per = 16 / size, shift = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / size;
   const int64_t stride = vocab + ((row_stride(logits) - vocab) % per + per) % per;
-  Tensor whole = at::empty({shift + n * stride}, logits.options());
+  Tensor whole = fresh({shift + n * stride}, logits.scalar_type(), logits);
   Tensor grad = whole.as_strided({n, vocab}, {stride, 1}, shift);
   ccl::LogprobBackwardParams p = {};
   p.logits = logits.data_ptr();
