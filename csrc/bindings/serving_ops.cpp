@@ -168,6 +168,7 @@ void check_cache(const char* op, const Tensor& like, const Tensor& k, const Tens
   TORCH_CHECK(ks.size(0) == k.size(0) && ks.size(1) == kv && vs.sizes() == ks.sizes(), op, ": scales must be [num_blocks, kv_heads]");
   TORCH_CHECK(kt.size(1) == kv && kt.size(2) == block && kt.size(3) == dim, op, ": tails must be [requests, kv_heads, block, head_dim]");
   TORCH_CHECK(k.size(0) * block <= 0x7fffffff && kt.size(0) <= 0x7fffffff, op, ": too many blocks or requests");
+  TORCH_CHECK(k.size(0) >= 1, op, ": a pool without pages");  // (what is not there is read from page 0, with a weight of zero)
   expect(cos, op, "cos", at::kFloat, 2, like);
   expect(sin, op, "sin", at::kFloat, 2, like);
   TORCH_CHECK(cos.size(1) == dim / 2 && sin.sizes() == cos.sizes() && cos.size(0) <= 0x7fffffff, op, ": cos and sin must be [positions, head_dim / 2]");

@@ -931,7 +931,7 @@ cudaError_t decode_attention8(const DecodeAttn8Params& p, cudaStream_t stream) {
   const KvCache8& c = p.cache;
   if (p.batch == 0) return cudaSuccess;
   if (p.batch < 0 || p.batch > 65535 || p.nsplit < 1 || c.n_kv_heads < 1 || p.n_heads < 1 || p.n_heads % c.n_kv_heads != 0 || p.n_heads > 65535) return cudaErrorInvalidValue;
-  if (c.block < 16 || c.block > 128 || (c.block & (c.block - 1)) != 0 || p.max_blocks < 1 || c.requests < p.batch) return cudaErrorInvalidValue;
+  if (c.block < 16 || c.block > 128 || (c.block & (c.block - 1)) != 0 || p.max_blocks < 1 || c.num_blocks < 1 || c.requests < p.batch) return cudaErrorInvalidValue;
   if (p.nsplit > 1 && !p.cluster && !p.partials) return cudaErrorInvalidValue;
   if (!aligned16(p.qkv) || !aligned16(c.k) || !aligned16(c.v) || !aligned16(c.k_tail) || !aligned16(c.v_tail) || !aligned16(p.out)) return cudaErrorInvalidValue;
   if (p.qkv_stride % 8 != 0 || p.out_stride % 8 != 0) return cudaErrorInvalidValue;

@@ -99,6 +99,14 @@ def test_cache_refuses():
             append(dict(a, cache=wrong))
 
 
+def test_a_pool_without_pages_is_refused():
+    a = make(num_blocks=0)
+    with pytest.raises(RuntimeError, match="a pool without pages"):
+        attend(a)
+    with pytest.raises(RuntimeError, match="a pool without pages"):
+        append(a)
+
+
 def test_append_refuses():
     a = make()
     with pytest.raises(RuntimeError, match="one for each row of qkv"):
