@@ -586,8 +586,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
   int n = 0;
   for (; n < n_pairs; ++n) {
     if ((n & 15) == 0) {
-      ks = ks_next;
-      lvs = log2f(vs_next);
+      // (an infinite scale, that of a page with an infinity, stands for 0 * inf in every position: NaN)
+      ks = ks_next + (ks_next - ks_next);
+      lvs = log2f(vs_next + (vs_next - vs_next));
       ivs = __frcp_rn(vs_next);
     }
     float s[NT][2][4], uiv[2];
@@ -693,7 +694,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
 #pragma unroll
     for (int a = 0; a < NT; ++a)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[a][0][e] = first + g + (e >> 1) * 8 <= place ? s[a][0][e] * fs : -INFINITY;
+      for (int e = 0; e < 4; ++e) {
+        // (what passes fp32 is NaN: the sign of its infinity may be that of a small part)
+        const float x = s[a][0][e] * fs + (s[a][0][e] - s[a][0][e]);
+        s[a][0][e] = first + g + (e >> 1) * 8 <= place ? x : -INFINITY;
+      }
     const float one[1] = {1.f};
     weigh(s, one);
     // two bf16 parts of the weights, the upper half of their bits and the rest, which is never zero: an infinity stays one
@@ -778,16 +783,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
       x0 += v.x * x;
       x1 += v.y * x;
     }
+    // (a sum below zero: a page outside the pool)
     if (sp.used == 1) {
       const float inv = 1.f / L;
       reinterpret_cast<uint32_t*>(out + (size_t)r * D)[d / 2] = any_bad ? 0 : pack_bf16(x0 * inv, x1 * inv);
     } else if (p.cluster) {
       sm.joined[r * (PR + 1) + d / 2] = make_float2(x0, x1);
-      if (d == 0) sm.joined[r * (PR + 1) + PR] = make_float2(any_bad ? INFINITY : M, L);
+      if (d == 0) sm.joined[r * (PR + 1) + PR] = make_float2(M, any_bad ? -1.f : L);
     } else {
       float* part = p.partials + (((size_t)b * p.n_heads + head0 + r) * p.nsplit + split) * (D + 2);
       *reinterpret_cast<float2*>(part + 2 + d) = make_float2(x0, x1);
-      if (d == 0) *reinterpret_cast<float2*>(part) = make_float2(any_bad ? INFINITY : M, L);
+      if (d == 0) *reinterpret_cast<float2*>(part) = make_float2(M, any_bad ? -1.f : L);
     }
   }
   if (sp.used == 1 || !p.cluster) return;
@@ -809,15 +815,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
     for (int k = 0; k < kMaxCluster; ++k)
       if (k < sp.used) M = fmaxf(M, ml[k].x);
     float L = 0.f, x0 = 0.f, x1 = 0.f;
+    bool zero = false;
 #pragma unroll
     for (int k = 0; k < kMaxCluster; ++k)
       if (k < sp.used) {
         const float w = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - M);
+        zero = zero || ml[k].y < 0.f;
         L += ml[k].y * w;
         x0 += x[k].x * w;
         x1 += x[k].y * w;
       }
-    reinterpret_cast<uint32_t*>(out + (size_t)r * D)[i % PR] = M == INFINITY ? 0 : pack_bf16(x0 / L, x1 / L);
+    reinterpret_cast<uint32_t*>(out + (size_t)r * D)[i % PR] = zero ? 0 : pack_bf16(x0 / L, x1 / L);
   }
   ptx::cluster_arrive();  // nobody leaves while its results are read
   ptx::cluster_wait();
@@ -837,14 +845,16 @@ __global__ void __launch_bounds__(D) merge_splits_kernel(const DecodeAttn8Params
   float M = -INFINITY;
   for (int i = 0; i < used; ++i) M = fmaxf(M, part[(size_t)i * (D + 2)]);
   float L = 0.f, acc = 0.f;
+  bool zero = false;
 #pragma unroll 4
   for (int i = 0; i < used; ++i) {
     const float* x = part + (size_t)i * (D + 2);
     const float w = x[0] == -INFINITY ? 0.f : exp2_fast(x[0] - M);
+    zero = zero || x[1] < 0.f;
     L += x[1] * w;
     acc += x[2 + d] * w;
   }
-  p.out[(size_t)b * p.out_stride + (size_t)h * D + d] = __float2bfloat16(M == INFINITY ? 0.f : acc / L);
+  p.out[(size_t)b * p.out_stride + (size_t)h * D + d] = __float2bfloat16(zero ? 0.f : acc / L);
 }
 
 constexpr int places(int tile) { return (tile == 1 ? 3 : 2) * 148; }  // CTAs that the GPU holds at a time

@@ -224,6 +224,38 @@ def test_nan_and_infinity_stay_where_they_are():
     assert torch.equal(out[2, 1, :, :5], want[2, 1, :, :5]) and torch.equal(out[2, 1, :, 6:], want[2, 1, :, 6:])
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("at", [100, 3000, 20000])
+def test_what_is_not_finite_is_not_a_number_in_every_split(at, dtype):
+    """A page with an infinity has an infinite scale, and 0 * inf in every position: NaN, in one split, a cluster's, or more. So have scores that
+    pass fp32. Not the zeros of a page outside the pool."""
+    for change in ("k", "v", "score"):
+        w = World([at, 40, at], 1, 4, 16, 128, dtype)
+        clean = World([at, 40, at], 1, 4, 16, 128, dtype)
+        want = attend(clean)
+        if change == "score":
+            w.qkv[2, :5 * 128] = 2.0**70  # q and the new k: their product is 2^147
+        else:
+            scale = w.cache.k_scale if change == "k" else w.cache.v_scale
+            scale[int(w.table[2, 3])] = float("inf")
+        out = attend(w)
+        assert torch.isnan(out[2]).all(), change
+        assert torch.equal(out[:2], want[:2])
+
+
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+def test_an_infinity_in_a_block_that_fills_up(dtype):
+    """In the tail it is the new token's own; once the block is a page, everything that reads it is NaN."""
+    for part in (0, 1):
+        w = World([31, 30], 1, 2, 16, 128, dtype)
+        w.cache[4 + part][0, 0, 3, 7] = float("inf")
+        attend(w)
+        assert torch.isinf(w.cache[2 + part][int(w.table[0, 1]), 0])
+        w.at, w.positions = [32, 31], i32([32, 31])
+        out = attend(w)
+        assert torch.isnan(out[0]).all() and not torch.isnan(out[1]).any()
+
+
 def test_pages_outside_the_pool():
     """Rows of zeros for a sequence with such a page, in the same split or another, and its token is still appended."""
     at = [100, 100, 3000, 15]
