@@ -353,7 +353,7 @@ long long row_stride(const Tensor& logits) { return logits.size(0) > 1 ? logits.
 
 using Logprobs = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 Logprobs logprob_shapes(int64_t rows, int64_t top, const Tensor& like) {
-  auto t = fresh_together<5>(like, {{{{rows}, at::kFloat}, {{rows}, at::kFloat}, {{rows}, at::kFloat}, {{rows, top}, at::kFloat}, {{rows, top}, at::kLong}}});
+  auto t = fresh_together<5>(like, {{{{rows}, at::kFloat}, {{rows}, at::kFloat}, {{rows, 2}, at::kFloat}, {{rows, top}, at::kFloat}, {{rows, top}, at::kLong}}});
   return {t[0], t[1], t[2], t[3], t[4]};
 }
 ccl::LogprobParams logprob_params(const Tensor& logits, const Tensor& targets, int64_t top, int64_t base, int64_t total) {
@@ -437,10 +437,10 @@ void check_backward(const Tensor& logits, const Tensor& targets, const Tensor& l
   TORCH_CHECK(top_ids.dim() == 2, op, ": top_ids must be [rows, top]");
   check_logits(op, logits, targets, top_ids.size(1), base, total);
   const int64_t n = logits.size(0);
-  expect(lse, op, "lse", at::kFloat, 1, logits);
+  expect(lse, op, "lse", at::kFloat, 2, logits);
   expect(entropy, op, "entropy", at::kFloat, 1, logits);
   expect(top_ids, op, "top_ids", at::kLong, 2, logits);
-  TORCH_CHECK(lse.size(0) == n && entropy.size(0) == n && top_ids.size(0) == n, op, ": lse, entropy and top_ids must have ", n, " rows");
+  TORCH_CHECK(lse.size(0) == n && lse.size(1) == 2 && entropy.size(0) == n && top_ids.size(0) == n, op, ": lse, entropy and top_ids must have ", n, " rows");
   if (g_lp) expect(*g_lp, op, "the gradient of logprob", at::kFloat, 1, logits);
   if (g_ent) expect(*g_ent, op, "the gradient of entropy", at::kFloat, 1, logits);
   if (g_top) expect(*g_top, op, "the gradient of top_logprobs", at::kFloat, 2, logits);

@@ -29,6 +29,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLag = 8.f;
+constexpr float kFar = 131072.f;  // rows whose maximum is larger go value by value: natural() is exact enough below
 constexpr int kMaxCluster = 16;
 constexpr int kClusterVecs = 1024;  // 16-byte vectors of a row for each CTA of its cluster, at least
 constexpr uint32_t kAbsent = 0xffffffffu;  // bits of "the target is in another shard"
@@ -118,11 +119,13 @@ __device__ __forceinline__ FastSums join(FastSums a, FastSums b) {
   a.t += b.t;
   return a;
 }
-// m to natural units; what its rounding leaves goes into the sums.
+// m to natural units, over the same rounded log2 e that the logits were multiplied with (at 2^20, ln 2 in its place is 2^-6 off); what its
+// rounding leaves goes into the sums.
 __device__ __forceinline__ Sums natural(const FastSums& a) {
-  constexpr float kLn2High = 0.693145752f, kLn2Low = 1.42860677e-6f;  // the upper 16 bits of ln 2, and the rest
-  const float high = a.m * kLn2High, low = a.m * kLn2Low;             // (the first is exact for |m| up to 2^8)
-  const float m = high + low, left = (fmaf(a.m, kLn2High, -high) + (high - m)) + low;
+  constexpr float kHigh = 0.693145752f;                                    // the upper 16 bits of 1 / kLog2e
+  constexpr float kLow = (float)(1.0 / (double)kLog2e - (double)kHigh);    // and the rest
+  const float high = a.m * kHigh, low = a.m * kLow;
+  const float m = high + low, left = (fmaf(a.m, kHigh, -high) + (high - m)) + low;
   const float f = 1.f + left + 0.5f * left * left;
   return {m, a.s * f, fmaf(left * kLog2e, a.s, a.t) * f};
 }
@@ -244,14 +247,15 @@ __device__ __forceinline__ Shape shape_of(const T* row, int vocab) {
 
 // What one thread writes when the sums of a row are known.
 struct RowResult {
-  float lse, logprob, entropy;
+  float m, log_s, logprob, entropy;  // log sum e^x = m + log_s: their sum in one number would lose 2^-24 of m
 };
 __device__ __forceinline__ RowResult finish(const Sums& a, long long target, long long total, float x_target) {
   RowResult r;
   const float log_s = logf(a.s);
-  r.lse = a.m + log_s;
+  r.m = a.m;
+  r.log_s = log_s;
   r.entropy = log_s - kLn2 * a.t / a.s;
-  r.logprob = target < 0 ? 0.f : (target >= total ? __int_as_float(0x7fc00000) : x_target - r.lse);
+  r.logprob = target < 0 ? 0.f : (target >= total ? __int_as_float(0x7fc00000) : (x_target - a.m) - log_s);
   return r;
 }
 
@@ -267,7 +271,7 @@ struct FwdSmem {
   unsigned long long bound;
   int n_threads, n_found;
   uint16_t threads[WARPS * 32];                    // those that may hold a candidate
-  float lse;
+  float m, log_s;
   bool special;
 };
 
@@ -436,7 +440,7 @@ __global__ void __launch_bounds__(WARPS * 32, 48 / WARPS) token_logprobs_kernel(
   if (tid == 0) {
     sum = cluster > 1 ? sm.rank[0] : sm.warp[0];
     for (int w = 1; w < cluster; ++w) sum = join(sum, sm.rank[w]);
-    sm.special = !(sum.s > 0.f && sum.s < INFINITY && fabsf(sum.t) < INFINITY && sum.m > Vec<T>::kLow);
+    sm.special = !(sum.s > 0.f && sum.s < INFINITY && fabsf(sum.t) < INFINITY && sum.m > Vec<T>::kLow && sum.m < kFar && sum.m > -kFar);
   }
   __syncthreads();
   if (sm.special) {  // the whole row once more, value by value
@@ -461,10 +465,11 @@ __global__ void __launch_bounds__(WARPS * 32, 48 / WARPS) token_logprobs_kernel(
       out[0] = sum.m, out[1] = sum.s, out[2] = sum.t, out[3] = xt;
     } else {
       const RowResult f = finish(sum, target, p.vocab_total, xt);
-      p.lse[r] = f.lse;
+      reinterpret_cast<float2*>(p.lse)[r] = make_float2(f.m, f.log_s);
       p.logprob[r] = f.logprob;
       p.entropy[r] = f.entropy;
-      sm.lse = f.lse;
+      sm.m = f.m;
+      sm.log_s = f.log_s;
     }
   }
   if constexpr (TOP) {
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(WARPS * 32, 48 / WARPS) token_logprobs_kernel(
         out[place] = k ? value_of(k) : -INFINITY;
         out[K + place] = __int_as_float(k ? (int)(p.vocab_base + index_of(k)) : -1);
       } else {
-        p.top_logprobs[(size_t)r * K + place] = value_of(k) - sm.lse;
+        p.top_logprobs[(size_t)r * K + place] = (value_of(k) - sm.m) - sm.log_s;
         p.top_ids[(size_t)r * K + place] = p.vocab_base + index_of(k);
       }
     }
@@ -500,7 +505,7 @@ __global__ void __launch_bounds__(WARPS * 32, 48 / WARPS) token_logprobs_kernel(
 constexpr int kMergeThreads = 128, kMaxShards = 64;
 __global__ void __launch_bounds__(kMergeThreads) merge_shards_kernel(const LogprobMergeParams p) {
   __shared__ unsigned long long keys[kMaxShards * kMaxTopLogprobs];
-  __shared__ float s_lse;
+  __shared__ float s_m, s_log_s;
   ptx::griddep_wait();
   const int r = blockIdx.x, tid = threadIdx.x, K = p.top, words = 4 + 2 * K;
   const float* mine = p.partials + (size_t)r * words;
@@ -516,7 +521,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_shards_kernel(const Logpr
       if (__float_as_uint(x[3]) != kAbsent) xt = x[3];
     }
     const RowResult f = finish(a, p.targets[r], p.vocab_total, xt);
-    p.lse[r] = s_lse = f.lse;
+    reinterpret_cast<float2*>(p.lse)[r] = make_float2(f.m, f.log_s);
+    s_m = f.m;
+    s_log_s = f.log_s;
     p.logprob[r] = f.logprob;
     p.entropy[r] = f.entropy;
   }
@@ -533,7 +540,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_shards_kernel(const Logpr
     int place = 0;
     for (int j = 0; j < n && place < K; ++j) place += keys[j] > k;
     if (place < K) {
-      p.top_logprobs[(size_t)r * K + place] = value_of(k) - s_lse;
+      p.top_logprobs[(size_t)r * K + place] = (value_of(k) - s_m) - s_log_s;
       p.top_ids[(size_t)r * K + place] = index_of(k);
     }
   }
@@ -543,10 +550,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_shards_kernel(const Logpr
 constexpr int kBwdThreads = 256, kBwdVecs = 4;
 
 struct RowGrad {
-  float lse, entropy, whole, g_entropy;
+  float m, log_s, entropy, whole, g_entropy;
 };
 __device__ __forceinline__ float grad_of(const RowGrad& g, float x) {
-  const float lp = x - g.lse, pr = ex2(lp * kLog2e);
+  const float lp = (x - g.m) - g.log_s, pr = ex2(lp * kLog2e);
   const float inner = g.whole + g.g_entropy * (lp + g.entropy);
   return pr == 0.f ? 0.f : -pr * inner;  // (-inf has no part in it)
 }
@@ -566,7 +573,8 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprobs_backward_kernel(co
 #pragma unroll
     for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     if (tid == 0) {
-      s_g.lse = p.lse[r];
+      s_g.m = p.lse[2 * r];
+      s_g.log_s = p.lse[2 * r + 1];
       s_g.entropy = p.entropy[r];
       s_g.whole = g_lp + sum;
       s_g.g_entropy = p.g_entropy ? p.g_entropy[r] : 0.f;

@@ -20,7 +20,7 @@ struct LogprobParams {
   // whole vocabulary
   float* logprob;            // [rows]
   float* entropy;
-  float* lse;
+  float* lse;                // [rows, 2]: a reference, and the logarithm of the sum of e^(x - reference)
   float* top_logprobs;       // [rows, top], best first; equal ones by id; a NaN is larger than everything
   long long* top_ids;
   // a shard (the five above are not written): [rows, 4 + 2 * top] words {max, sum, weighted sum, target's logit, values.., ids (int32)..}
@@ -50,7 +50,7 @@ struct LogprobBackwardParams {
   int rows, vocab, top;
   const long long* targets;
   long long vocab_base, vocab_total;
-  const float* lse;
+  const float* lse;          // [rows, 2]
   const float* entropy;
   const long long* top_ids;  // [rows, top]
   const float* g_logprob;    // [rows]

@@ -209,6 +209,33 @@ def test_gradient_of_strided_rows(dtype, offset, pad):
         assert (base.grad[:, :offset] == 0).all() and (base.grad[:, offset + vocab:] == 0).all()
 
 
+@pytest.mark.parametrize("offset", [2.0**7, -(2.0**10), 2.0**14, -(2.0**17), 2.0**20, 2.0**23])
+@pytest.mark.parametrize("vocab", [1000, 32003])
+def test_a_common_offset_of_a_row_takes_nothing(vocab, offset):
+    """Differences of fp32 logits are exact, wherever they lie: the bounds are those of the logits without the offset (of up to 20, and 2^-40 of the
+    offset for the two parts that a base-2 reference is turned to natural units with)."""
+    x, t = inputs(5, vocab, F32, vocab)
+    x = (x + offset).requires_grad_(True)
+    got = ops.token_logprobs(x, t, 4)
+    ref = torch.log_softmax(x.detach().double(), -1)
+    e, far = tol(vocab), abs(offset) * 2.0**-40
+    lp = ref.gather(1, t[:, None])[:, 0]
+    assert ((got.logprob.double() - lp).abs() <= e + 40 * 2.0**-22 + far).all()
+    assert ((got.entropy.double() + (ref.exp() * ref).sum(-1)).abs() <= 31 * e).all()
+    assert ((got.top_logprobs.double() - ref.gather(1, got.top_ids)).abs() <= e + 40 * 2.0**-22 + far).all()
+    g = torch.randn(5, device="cuda"), torch.randn(5, device="cuda"), torch.randn(5, 4, device="cuda")
+    d, = torch.autograd.grad([got.logprob, got.entropy, got.top_logprobs], x, g)
+    want, size = grad_ref(x.detach(), t, got.top_ids, *g)
+    p = ref.exp()
+    assert ((d.double() - want).abs() <= want.abs() * 2.0**-23 + size + p * far * 100).all()
+    # two shards of the vocabulary, joined
+    half = vocab // 2
+    if 2 * half == vocab:
+        parts = torch.stack([torch.ops.ccl.token_logprobs_shard(x.detach()[:, i * half:(i + 1) * half], t, 4, i * half, vocab) for i in range(2)])
+        joined = torch.ops.ccl.token_logprobs_merge(parts, t, 4, vocab)
+        assert ((joined[0].double() - lp).abs() <= 2 * e + 40 * 2.0**-22 + far).all()
+
+
 @pytest.mark.parametrize("shards,vocab,top", [(2, 500, 5), (4, 40, 32), (8, 4000, 20), (8, 3, 20), (2, 16001, 0), (64, 8, 32)])
 def test_shards_of_a_vocabulary(shards, vocab, top):
     """The shards' results, joined, are the whole vocabulary's; so are their gradients."""
