@@ -257,7 +257,8 @@ Tensor kv_append_8bit_meta(const Tensor& qkv, PLAN_ARGS, CACHE_ARGS, const Tenso
 }
 void kv_append_8bit_out_cuda(const Tensor& qkv, PLAN_ARGS, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads, Tensor& out) {
   check_append(qkv, starts, requests, positions, slots, k, v, ks, vs, kt, vt, cos, sin, n_heads, &out);
-  TORCH_CHECK(!overlap(qkv, out), "kv_append_8bit: out shares memory with qkv");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&qkv, &k, &v, &kt, &vt})
+    TORCH_CHECK(!overlap(*t, out), "kv_append_8bit: out shares memory with qkv or the cache");
   c10::cuda::CUDAGuard g(qkv.device());
   append(qkv, starts, requests, positions, slots, k, v, ks, vs, kt, vt, cos, sin, n_heads, out, false);
 }
@@ -326,7 +327,8 @@ Tensor decode_attention_8bit_meta(const Tensor& qkv, const Tensor& positions, co
 }
 void decode_attention_8bit_out_cuda(const Tensor& qkv, const Tensor& positions, const Tensor& table, CACHE_ARGS, const Tensor& cos, const Tensor& sin, int64_t n_heads, Tensor& out) {
   check_attention(qkv, positions, table, k, v, ks, vs, kt, vt, cos, sin, n_heads, &out);
-  TORCH_CHECK(!overlap(qkv, out), "decode_attention_8bit: out shares memory with qkv");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&qkv, &k, &v, &kt, &vt})
+    TORCH_CHECK(!overlap(*t, out), "decode_attention_8bit: out shares memory with qkv or the cache");
   c10::cuda::CUDAGuard g(qkv.device());
   attention(qkv, positions, table, k, v, ks, vs, kt, vt, cos, sin, n_heads, out);
 }

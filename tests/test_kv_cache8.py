@@ -180,6 +180,17 @@ def test_rows_with_strides_and_a_given_result():
         attend(w, out=room[:, 4:-12])
 
 
+def test_a_result_in_the_cache_is_refused():
+    w = World([100, 31, 5], 2, 4, 32, 128, E4M3)
+    plan = ops.kv_plan(i32([0, 0, 0]), i32([1, 1, 1]), ops.KVBlocks.empty(3, 4, w.cache.k.shape[0]), 32, 3)
+    for tail in w.cache[4:]:
+        rows = tail.view(3, -1)
+        with pytest.raises(RuntimeError, match="shares memory"):
+            attend(w, out=rows[:, :w.heads * 128])
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.kv_append_8bit(w.qkv, plan, w.cache, w.cos, w.sin, w.heads, out=rows[:, :(w.heads + 2) * 128])
+
+
 def test_scales_of_every_size():
     """Pages whose V scales differ by 2^40: weights are kept relative to what they contribute."""
     w = World([321, 95], 2, 4, 16, 128, I8)

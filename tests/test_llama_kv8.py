@@ -89,6 +89,15 @@ def test_capture_leaves_the_sequences_as_they_were():
         assert torch.equal(a.decode_step(4), b.decode_step(4)) and torch.equal(a.logits, b.logits)
 
 
+def test_log_probabilities_after_a_capture_are_those_of_the_first_replay():
+    m = _model("fp8", kv_block=16, logprobs=2)
+    m.prefill(_prompt(4, 20))
+    m.capture(4)
+    assert m.last_logprobs is None  # nothing has run that could give any
+    m.decode_step(4)
+    assert torch.equal(m.last_logprobs.top_ids[:, 0], m.next_tokens[:4].long()) and (m.last_logprobs.logprob <= 0).all()
+
+
 def test_sequences_end_and_others_take_their_pages():
     m = _model("fp8", kv_block=16, kv_blocks=4 * 4 + 2)
     m.prefill(_prompt(4, 60))

@@ -375,6 +375,7 @@ class TPLlamaDecoder:
         with torch.cuda.graph(g, stream=s):
             self._decode_body(B)
         self.graph, self.graph_batch, self.graph_logprobs = g, B, self.last_logprobs
+        self.last_logprobs = None  # nothing is in the graph's before its first replay
         torch.cuda.synchronize(self.device)
         return g
 
