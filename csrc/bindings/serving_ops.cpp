@@ -3,6 +3,7 @@
 // Each op has one function that checks its arguments and gives its results' shapes, which the CUDA and the Meta kernel share, so that
 // tracing refuses what a launch would refuse.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -448,10 +449,19 @@ void check_backward(const Tensor& logits, const Tensor& targets, const Tensor& l
   if (g_top) expect(*g_top, op, "the gradient of top_logprobs", at::kFloat, 2, logits);
   TORCH_CHECK((!g_lp || g_lp->size(0) == n) && (!g_ent || g_ent->size(0) == n) && (!g_top || g_top->sizes() == top_ids.sizes()), op, ": gradients must have the results' sizes");
 }
+// A backward pass in a graph's capture, of a leaf that an eager graph still holds: the engine would let the default stream, where that one's
+// gradients are accumulated, wait for the capturing one, which ends the capture and with it the process.
+void refuse_held_leaf(const Tensor& logits) {
+  if (!logits.requires_grad() || !logits.is_leaf() || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(logits);
+  const auto at = accumulator ? accumulator->stream() : c10::nullopt;
+  TORCH_CHECK(!at || at->id() != 0, "token_logprobs: backward in a graph's capture while results of the same logits from the default stream are alive: delete those before");
+}
 Tensor token_logprobs_backward_cuda(const Tensor& logits, const Tensor& targets, const Tensor& lse, const Tensor& entropy, const Tensor& top_ids, const optional<Tensor>& g_lp,
                                     const optional<Tensor>& g_ent, const optional<Tensor>& g_top, int64_t base, int64_t total) {
   check_backward(logits, targets, lse, entropy, top_ids, g_lp, g_ent, g_top, base, total);
   c10::cuda::CUDAGuard g(logits.device());
+  refuse_held_leaf(logits);
   const int64_t n = logits.size(0), vocab = logits.size(1), size = logits.element_size();
   // the gradient's rows lie as the logits' rows do relative to 16 bytes, so that one vector of the one is one of the other
   const int64_t per = 16 / size, shift = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / size;

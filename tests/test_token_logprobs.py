@@ -298,6 +298,27 @@ def test_step_captured_with_its_gradient():
     assert torch.equal(d, want)
 
 
+def test_a_captured_gradient_of_a_leaf_that_an_eager_graph_holds_is_refused():
+    x, t = inputs(64, 2000, BF16)
+    x.requires_grad_(True)
+    held = ops.token_logprobs(x, t)  # on the default stream
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="delete those before"):
+        with torch.cuda.graph(graph, stream=s):
+            torch.autograd.grad(ops.token_logprobs(x, t).logprob.sum(), x)
+    torch.cuda.synchronize()
+    want, = torch.autograd.grad(held.logprob.sum(), x)
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        d, = torch.autograd.grad(ops.token_logprobs(x, t).logprob.sum(), x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(d, want)
+
+
 def test_group_of_one_rank():
     import torch.distributed as dist
 

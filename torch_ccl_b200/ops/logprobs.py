@@ -52,7 +52,8 @@ def token_logprobs(logits, targets, top=0, group=None):
     a `TokenLogprobs`, differentiable in the logits (bf16, fp16 or fp32 [rows, vocabulary]; rows may be strided).
 
     targets: int64 [rows]; a negative one stands for "no token" (log-probability 0, no gradient from it), one past the vocabulary gives NaN.
-    Equal logits are ordered by id; a NaN counts as larger than everything, as in torch.topk. Sums are in fp32.
+    Equal logits are ordered by id; a NaN counts as larger than everything, as in torch.topk. Sums are in fp32. A gradient may
+    be captured in a graph if no result of the same logits (where they are a leaf) from the default stream is alive; one that is, is an error.
 
     group: `logits` are this rank's equal shard of the vocabulary (rank 0 has the first ids); every rank passes the same targets, gets
     the whole vocabulary's results, and the gradient of its own shard. None: `logits` have the whole vocabulary."""
