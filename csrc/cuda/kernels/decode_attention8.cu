@@ -28,11 +28,12 @@ namespace {
 
 using namespace kv8;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+// CTAs of 3, 4 or 6 warps (W): the GPU holds 592, 444 or 296 of them, twelve warps an SM. With sixteen query rows (NT 2) a warp's state takes
+// twice the registers: CTAs of four, two an SM.
+constexpr int ctas_per_sm(int NT, int W) { return NT == 1 ? 12 / W : 2; }
 constexpr int kStages = 2;         // pairs of units on their way to a warp, or in use
 constexpr int kMaxSplits = 64, kMaxCluster = 16;
-constexpr int kLeast = 8;          // units of 16 positions per split at least: a pair for each warp
+constexpr int least_units(int W) { return 2 * W; }  // units of 16 positions per split at least: a pair for each warp
 constexpr int kChunk = 512;        // units of a split where there are CTAs enough without splits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHead = 8.f;       // the reference starts this far (log2) below the maximum
@@ -74,6 +75,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float f16_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
+__device__ __forceinline__ float f16_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -125,7 +128,7 @@ __device__ __forceinline__ void widen_biased(uint32_t w, uint32_t& lo, uint32_t&
   hi = *reinterpret_cast<const uint32_t*>(&y);
 }
 
-template <int D, int NT>
+template <int D, int NT, int W>
 struct Smem {
   static constexpr int R = 8 * NT;       // query rows
   static constexpr int QP = D + 4;       // pitch (halves): eight rows start two banks apart
@@ -133,9 +136,9 @@ struct Smem {
   static constexpr int OP = 8 * OS + 2;  // pitch (floats)
   static constexpr int kUnit = 16 * D;   // bytes of K, or of V, of a unit of 16 positions
   union {
-    uint8_t ring[kWarps][kStages][2][2 * kUnit];  // K and V of two units
+    uint8_t ring[W][kStages][2][2 * kUnit];  // K and V of two units
     struct {                             // at the end
-      float o[kWarps][R * OP];           // out of each warp
+      float o[W][R * OP];           // out of each warp
       float2 joined[R * (D / 2 + 1)];    // of the CTA, for the others of its cluster: out, and {m, l} behind each row
     };
   };
@@ -144,14 +147,13 @@ struct Smem {
       __half qh[R * QP], ql[R * QP];     // q as two f16 parts
     };
     struct {
-      float m[kWarps][R], l[kWarps][R];  // at the end
+      float m[W][R], l[W][R];  // at the end
     };
   };
-  __nv_bfloat16 qb[3][R * QP];           // q as three bf16 parts, for the tail
   float qs[R];                           // scale * log2 e over the power of two of the row
   float qc[R];                           // int8: what the codes' bias adds to a score
   uint4 new_k[D / 8], new_v[D / 8];      // the new token, bf16
-  uint32_t amax[2][kWarps];
+  uint32_t amax[2][W];
   int bad;
 };
 
@@ -170,7 +172,6 @@ __device__ __forceinline__ NewToken load_new(const DecodeAttn8Params& p, int b, 
 }
 template <int D>
 __device__ __forceinline__ void store_new(const DecodeAttn8Params& p, NewToken w, int pos, uint4* k, uint4* v) {
-  static_assert(kThreads >= D / 2, "a thread for each pair of words of k, and of v");
   const int tid = threadIdx.x, i = tid & (D / 4 - 1);
   if (tid >= D / 2) return;
   if (tid < D / 4) {  // dims 2i and 2i + 1 and the ones half a head further on
@@ -188,8 +189,9 @@ __device__ __forceinline__ void store_new(const DecodeAttn8Params& p, NewToken w
 
 // Quantises the block that the new token completes. A CTA of its own does that, beside the attention (which reads this block from the
 // tail): within the CTA that attends it took as long as 300 positions.
-template <int D, bool INT8>
-__device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b, int kvh, uint4* fresh_k, uint4* fresh_v, uint32_t (*amax)[kWarps]) {
+template <int D, bool INT8, int W>
+__device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b, int kvh, uint4* fresh_k, uint4* fresh_v, uint32_t (*amax)[W]) {
+  constexpr int kThreads = W * 32;
   const KvCache8& c = p.cache;
   const int tid = threadIdx.x, pos = p.positions[b];
   if (!position_ok(p, pos) || (pos & (c.block - 1)) != c.block - 1) return;
@@ -226,7 +228,7 @@ __device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b
   if ((tid & 31) == 0) amax[0][tid >> 5] = seen_k, amax[1][tid >> 5] = seen_v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) seen_k = max(seen_k, amax[0][w]), seen_v = max(seen_v, amax[1][w]);
+  for (int w = 0; w < W; ++w) seen_k = max(seen_k, amax[0][w]), seen_v = max(seen_v, amax[1][w]);
   const float scale_k = scale_of<INT8>(bits_f(seen_k)), scale_v = scale_of<INT8>(bits_f(seen_v));
   uint2* to_k = reinterpret_cast<uint2*>(c.k + sc * c.block * D);
   uint2* to_v = reinterpret_cast<uint2*>(c.v + sc * c.block * D);
@@ -251,13 +253,13 @@ __device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b
   }
 }
 
-template <int D, int NT, bool INT8>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_kernel(const DecodeAttn8Params p) {
-  constexpr int R = 8 * NT;
+template <int D, int NT, bool INT8, int W>
+__global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_kernel(const DecodeAttn8Params p) {
+  constexpr int R = 8 * NT, kThreads = W * 32;
   constexpr int KJ = D / 64;        // 16-byte loads of a K row by a thread
   constexpr int VW = D / 32;        // words of a V row by a thread
   constexpr int NM = D / 16;        // products over the dims
-  using S = Smem<D, NT>;
+  using S = Smem<D, NT, W>;
   extern __shared__ __align__(16) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
 
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
   const int pair = blockIdx.x / p.nsplit, split = blockIdx.x - pair * p.nsplit;
   if (pair >= pairs) {
     const int i = (pair - pairs) * p.nsplit + split;
-    if (i < p.batch * c.n_kv_heads) quantise_block<D, INT8>(p, i % p.batch, i / p.batch, sm.new_k, sm.new_v, sm.amax);
+    if (i < p.batch * c.n_kv_heads) quantise_block<D, INT8, W>(p, i % p.batch, i / p.batch, sm.new_k, sm.new_v, sm.amax);
     return;
   }
   const int b = pair % p.batch, kvh = pair / p.batch / tiles, tile = pair / p.batch - kvh * tiles;
@@ -281,10 +283,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
   const int head0 = kvh * group + tile * R;
   const int pos = p.positions[b];
   // what needs no position is asked for with it: q (LPR lanes share a row; a lane has two words of it, half a head apart), the new token
-  constexpr int LPR = D / 4, RPW = 32 / LPR, QI = R / (kWarps * RPW);
+  constexpr int LPR = D / 4, RPW = 32 / LPR, QI = (R + W * RPW - 1) / (W * RPW);
   const int q_word = lane % LPR;
   uint32_t q_lo[QI], q_hi[QI];
-  auto q_row = [&](int i) { return (i * kWarps + warp) * RPW + lane / LPR; };
+  auto q_row = [&](int i) { return (i * W + warp) * RPW + lane / LPR; };
 #pragma unroll
   for (int i = 0; i < QI; ++i) {
     q_lo[i] = q_hi[i] = 0;
@@ -306,19 +308,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
   const bool owns_tail = split == sp.used - 1;
   const int* table = p.table + (size_t)b * p.max_blocks;
 
-  // ---- the loop's loads: units of the split in pairs, pair n of this warp being pair warp + 4 n -----------------------------------
+  // ---- the loop's loads: units of the split in pairs, pair n of this warp being pair warp + W n -----------------------------------
   const int u0 = split * sp.per, units = max(0, min(sp.units - u0, sp.per));
-  const int n_pairs = max(0, ((units + 1) / 2 - warp + kWarps - 1) / kWarps);
+  const int n_pairs = max(0, ((units + 1) / 2 - warp + W - 1) / W);
   const int in_block = 31 - __clz(c.block / 16);  // log2 of the units of a block
   const int place = pos & (c.block - 1);
   // the tail's units of 16 positions follow the pairs, the first of them with the last warp
   const int tail_units = owns_tail ? place / 16 + 1 : 0;
-  const int n_all = n_pairs + max(0, (tail_units - (kWarps - 1 - warp) + kWarps - 1) / kWarps);
-  auto tail_first = [&](int n) { return ((kWarps - 1 - warp) + kWarps * (n - n_pairs)) * 16; };
+  const int n_all = n_pairs + max(0, (tail_units - (W - 1 - warp) + W - 1) / W);
+  auto tail_first = [&](int n) { return ((W - 1 - warp) + W * (n - n_pairs)) * 16; };
   const size_t tail_at = ((size_t)b * c.n_kv_heads + kvh) * c.block * D;
   bool bad = false;
   // a window of 16 pairs: each lane looks up the page of one unit, and its scales
-  auto unit_of = [&](int n, int h) { return 2 * (warp + kWarps * n) + h; };
+  auto unit_of = [&](int n, int h) { return 2 * (warp + W * n) + h; };
   auto page_of = [&](int n) {  // of window n / 16, for this lane
     const int u = unit_of(n + (lane >> 1), lane & 1);
     if (u >= units) return 0;
@@ -429,24 +431,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int at = r * S::QP + h * (D / 2) + 2 * q_word;
+      const bool row = R % (W * RPW) == 0 || r < R;
       const __half2 hi = __floats2half2_rn(z[h][0] * to_f16, z[h][1] * to_f16);
       const __half2 lo = __floats2half2_rn(z[h][0] * to_f16 - __low2float(hi), z[h][1] * to_f16 - __high2float(hi));
-      *reinterpret_cast<__half2*>(&sm.qh[at]) = hi;
-      *reinterpret_cast<__half2*>(&sm.ql[at]) = lo;
-      sum += (__low2float(hi) + __low2float(lo)) + (__high2float(hi) + __high2float(lo));
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const uint32_t part = pack_bf16(z[h][0], z[h][1]);
-        *reinterpret_cast<uint32_t*>(&sm.qb[k][at]) = part;
-        z[h][0] -= lo_f(part);
-        z[h][1] -= hi_f(part);
+      if (row) {
+        *reinterpret_cast<__half2*>(&sm.qh[at]) = hi;
+        *reinterpret_cast<__half2*>(&sm.ql[at]) = lo;
       }
+      sum += (__low2float(hi) + __low2float(lo)) + (__high2float(hi) + __high2float(lo));
     }
     if constexpr (INT8) {
 #pragma unroll
       for (int x = LPR / 2; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     }
-    if (q_word == 0) {
+    if (q_word == 0 && r < R) {
       sm.qs[r] = p.scale * kLog2e / mult;
       sm.qc[r] = 128.f * sum * (p.scale * kLog2e / mult);
     }
@@ -667,7 +665,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
   }
 
   // ---- the tail, q in three bf16 parts and the weights in two ------------------------------------------------------------------------
-  const float fs = p.scale * kLog2e;
   for (; n < n_all; ++n) {
     const int first = tail_first(n);
     const uint4* stage = reinterpret_cast<const uint4*>(&sm.ring[warp][0][0][0] + (n % kStages) * 4 * S::kUnit) + lane;
@@ -683,12 +680,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
+        for (int a = 0; a < NT; ++a) {
+          const int at = (a * 8 + g) * S::QP + j * 32 + t * 8 + w * 4;
+          const uint2 hi = *reinterpret_cast<const uint2*>(&sm.qh[at]), lo = *reinterpret_cast<const uint2*>(&sm.ql[at]);
+          float z[4] = {f16_lo(hi.x) + f16_lo(lo.x), f16_hi(hi.x) + f16_hi(lo.x), f16_lo(hi.y) + f16_lo(lo.y), f16_hi(hi.y) + f16_hi(lo.y)};
+          uint32_t part[3][2];
 #pragma unroll
-          for (int i = 2; i >= 0; --i) {  // the small parts first
-            const uint2 q = *reinterpret_cast<const uint2*>(&sm.qb[i][(a * 8 + g) * S::QP + j * 32 + t * 8 + w * 4]);
-            mma_bf16(s[a][0], r0[2 * w], r8[2 * w], r0[2 * w + 1], r8[2 * w + 1], q.x, q.y);
-          }
+          for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // (the dims that e4m3's K has 2^-8 of)
+              if (i == 0 && !INT8 && w == 1) z[2 * e] *= 1.f / kLowE4m3, z[2 * e + 1] *= 1.f / kLowE4m3;
+              part[i][e] = pack_bf16(z[2 * e], z[2 * e + 1]);
+              z[2 * e] -= lo_f(part[i][e]);
+              z[2 * e + 1] -= hi_f(part[i][e]);
+            }
+#pragma unroll
+          for (int i = 2; i >= 0; --i) mma_bf16(s[a][0], r0[2 * w], r8[2 * w], r0[2 * w + 1], r8[2 * w + 1], part[i][0], part[i][1]);  // the small parts first
+        }
     }
     load_k(n + kStages, where);
 #pragma unroll
@@ -696,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // (what passes fp32 is NaN: the sign of its infinity may be that of a small part)
-        const float x = s[a][0][e] * fs + (s[a][0][e] - s[a][0][e]);
+        const float x = s[a][0][e] * (f[a][e & 1] * (INT8 ? 1.f / kLowInt8 : 1.f)) + (s[a][0][e] - s[a][0][e]);
         s[a][0][e] = first + g + (e >> 1) * 8 <= place ? x : -INFINITY;
       }
     const float one[1] = {1.f};
@@ -767,16 +776,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) decode_attention8_k
   __syncthreads();
   const bool any_bad = sm.bad != 0;
   constexpr int PR = D / 2;  // pairs of dims of a row
-  static_assert(kThreads % PR == 0 || PR % kThreads == 0, "whole rows");
 #pragma unroll 4
   for (int i = tid; i < rows * PR; i += kThreads) {
     const int r = i / PR, d = 2 * (i % PR);
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][r]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm.m[w][r]);
     float L = 0.f, x0 = 0.f, x1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float x = sm.m[w][r] == -INFINITY ? 0.f : exp2_fast(sm.m[w][r] - M);
       const float2 v = *reinterpret_cast<const float2*>(&sm.o[w][r * S::OP + d / (D / 8) * S::OS + d % (D / 8)]);
       L += sm.l[w][r] * x;
@@ -857,14 +865,12 @@ __global__ void __launch_bounds__(D) merge_splits_kernel(const DecodeAttn8Params
   p.out[(size_t)b * p.out_stride + (size_t)h * D + d] = __float2bfloat16(zero ? 0.f : acc / L);
 }
 
-constexpr int places(int tile) { return (tile == 1 ? 3 : 2) * 148; }  // CTAs that the GPU holds at a time
-
-template <int D, int NT, bool INT8>
+template <int D, int NT, bool INT8, int W>
 cudaError_t launch(const DecodeAttn8Params& p, cudaStream_t stream) {
-  auto kern = decode_attention8_kernel<D, NT, INT8>;
+  auto kern = decode_attention8_kernel<D, NT, INT8, W>;
   static DeviceOnce configured;
   if (configured.pending()) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT>));
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, NT, W>));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     configured.done();
@@ -875,8 +881,8 @@ cudaError_t launch(const DecodeAttn8Params& p, cudaStream_t stream) {
   if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Smem<D, NT>);
+  cfg.blockDim = dim3(W * 32);
+  cfg.dynamicSmemBytes = sizeof(Smem<D, NT, W>);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
@@ -884,7 +890,7 @@ cudaError_t launch(const DecodeAttn8Params& p, cudaStream_t stream) {
   // have two and others none: 264 of them for 33 ragged sequences take 44.8 us behind themselves, and 35.6 without. Calls of short pieces
   // and ones that fill the GPU gain what the placing hides (launched one by one: a sequence of 1000 8.8 instead of 10.2 us, 16 of 1087
   // with 512 CTAs 42.8 instead of 45.0).
-  const bool short_pieces = (long long)p.max_blocks * p.cache.block <= 512LL * p.nsplit, full = pairs * p.nsplit >= places(NT);
+  const bool short_pieces = (long long)p.max_blocks * p.cache.block <= 512LL * p.nsplit, full = pairs * p.nsplit >= 148 * ctas_per_sm(NT, W);
   cfg.numAttrs = short_pieces || full ? pdl_launch_attr(&attr[0]) : 0;
   if (p.cluster) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
@@ -905,13 +911,14 @@ cudaError_t launch(const DecodeAttn8Params& p, cudaStream_t stream) {
   if (e == cudaSuccess) launch_count_add(1);
   return e;
 }
-template <int D, int NT>
+template <int D, int NT, int W>
 cudaError_t by_code(const DecodeAttn8Params& p, cudaStream_t s) {
-  return p.cache.int8 ? launch<D, NT, true>(p, s) : launch<D, NT, false>(p, s);
+  return p.cache.int8 ? launch<D, NT, true, W>(p, s) : launch<D, NT, false, W>(p, s);
 }
 template <int D>
-cudaError_t by_tile(const DecodeAttn8Params& p, cudaStream_t s) {
-  return p.n_heads / p.cache.n_kv_heads > 8 ? by_code<D, 2>(p, s) : by_code<D, 1>(p, s);
+cudaError_t by_shape(const DecodeAttn8Params& p, cudaStream_t s) {
+  if (p.n_heads / p.cache.n_kv_heads > 8) return by_code<D, 2, 4>(p, s);
+  return p.warps == 3 ? by_code<D, 1, 3>(p, s) : (p.warps == 4 ? by_code<D, 1, 4>(p, s) : by_code<D, 1, 6>(p, s));
 }
 
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
@@ -923,13 +930,29 @@ void decode_attention8_split(DecodeAttn8Params& p) {
   const int tile = group > 8 ? 2 : 1, r = 8 * tile;  // query rows of a CTA
   const long long pairs = (long long)p.batch * p.cache.n_kv_heads * ((group + r - 1) / r);
   const long long units = (long long)p.max_blocks * (p.cache.block / 16);  // at most; how long the sequences are only the GPU knows
-  // As many CTAs as the GPU holds at a time, or, where there are more pairs than that, splits of kChunk units; none shorter than kLeast.
-  const long long want = pairs <= places(tile) ? places(tile) / pairs : (units + kChunk - 1) / kChunk;
-  p.nsplit = (int)std::max(1ll, std::min({want, (long long)kMaxSplits, (units + kLeast - 1) / kLeast}));
-  p.least = pairs <= places(tile) ? kLeast : kChunk;
-  // The CTAs of a sequence are a cluster, which joins their results without a second launch, unless there is so much for so few heads
-  // that more of them pay.
-  if (p.nsplit > kMaxCluster && units <= kMaxCluster * 64) p.nsplit = kMaxCluster;
+  double best = 0;
+  long long best_waves = 0;
+  for (int W : {6, 4, 3}) {
+    if (tile == 2 && W != 4) continue;
+    const int places = 148 * ctas_per_sm(tile, W);
+    // As many CTAs as the GPU holds at a time, or, where there are more pairs than that, splits of kChunk units; none shorter than a pair of
+    // units for each warp.
+    const int least = pairs <= places ? least_units(W) : kChunk;
+    const long long want = pairs <= places ? places / pairs : (units + kChunk - 1) / kChunk;
+    int nsplit = (int)std::max(1ll, std::min({want, (long long)kMaxSplits, (units + least - 1) / least}));
+    // The CTAs of a sequence are a cluster, which joins their results without a second launch, unless there is so much for so few heads
+    // that more of them pay.
+    if (nsplit > kMaxCluster && units <= kMaxCluster * 64) nsplit = kMaxCluster;
+    const long long ctas = pairs * nsplit, waves = (ctas + places - 1) / places;
+    const double fill = (double)ctas / (double)(waves * places);
+    if (fill > best + 1e-9 || (fill > best - 1e-9 && waves < best_waves)) {
+      best = fill;
+      best_waves = waves;
+      p.warps = W;
+      p.nsplit = nsplit;
+      p.least = least;
+    }
+  }
   p.cluster = p.nsplit > 1 && p.nsplit <= kMaxCluster;
 }
 
@@ -945,8 +968,8 @@ cudaError_t decode_attention8(const DecodeAttn8Params& p, cudaStream_t stream) {
   if (p.nsplit > 1 && !p.cluster && !p.partials) return cudaErrorInvalidValue;
   if (!aligned16(p.qkv) || !aligned16(c.k) || !aligned16(c.v) || !aligned16(c.k_tail) || !aligned16(c.v_tail) || !aligned16(p.out)) return cudaErrorInvalidValue;
   if (p.qkv_stride % 8 != 0 || p.out_stride % 8 != 0) return cudaErrorInvalidValue;
-  if (c.head_dim == 128) return by_tile<128>(p, stream);
-  if (c.head_dim == 64) return by_tile<64>(p, stream);
+  if (c.head_dim == 128) return by_shape<128>(p, stream);
+  if (c.head_dim == 64) return by_shape<64>(p, stream);
   return cudaErrorInvalidValue;
 }
 

@@ -57,7 +57,7 @@ struct DecodeAttn8Params {
   long long out_stride;
   float* partials;           // decode_attention8_partial_floats() floats; unused when there is one split
   int batch, n_heads, max_blocks, table_rows;
-  int nsplit, least;  // set by decode_attention8_split()
+  int nsplit, least, warps;  // set by decode_attention8_split()
   bool cluster;
   float scale;               // 1 / sqrt(head_dim)
   KvCache8 cache;

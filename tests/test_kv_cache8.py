@@ -160,6 +160,16 @@ def test_many_sequences_without_a_split():
     World([(i * 37) % 200 for i in range(700)], 4, 1, 16, 64, E4M3).check(attend)
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch", [74, 111, 148, 200])
+def test_attention_in_ctas_of_every_size(batch, dim, dtype):
+    """296, 444 and 592 pairs of a sequence and a KV head fill the GPU with CTAs of six, four and three warps; 800 do not fit at once."""
+    g = torch.Generator().manual_seed(batch)
+    at = EDGES + torch.randint(0, 500, (batch - len(EDGES),), generator=g).tolist()
+    World(at, 4, 3, 32, dim, dtype, seed=batch).check(attend)
+
+
 def test_rows_with_strides_and_a_given_result():
     w = World([100, 31, 5], 2, 4, 32, 128, E4M3)
     wide = torch.full((3, w.qkv.shape[1] + 24), float("nan"), device="cuda", dtype=BF16)
