@@ -171,11 +171,10 @@ __device__ __forceinline__ NewToken load_new(const DecodeAttn8Params& p, int b, 
   return {src[0], src[D / 4]};
 }
 template <int D>
-__device__ __forceinline__ void store_new(const DecodeAttn8Params& p, NewToken w, int pos, uint4* k, uint4* v) {
+__device__ __forceinline__ void store_new(NewToken w, float2 c, float2 s, uint4* k, uint4* v) {  // c, s: of dims 2i and 2i + 1
   const int tid = threadIdx.x, i = tid & (D / 4 - 1);
   if (tid >= D / 2) return;
   if (tid < D / 4) {  // dims 2i and 2i + 1 and the ones half a head further on
-    const float2 c = reinterpret_cast<const float2*>(p.cos + (size_t)pos * (D / 2))[i], s = reinterpret_cast<const float2*>(p.sin + (size_t)pos * (D / 2))[i];
     float x0, y0, x1, y1;
     rotate(lo_f(w.a), lo_f(w.b), c.x, s.x, x0, y0);
     rotate(hi_f(w.a), hi_f(w.b), c.y, s.y, x1, y1);
@@ -197,7 +196,8 @@ __device__ __forceinline__ void quantise_block(const DecodeAttn8Params& p, int b
   if (!position_ok(p, pos) || (pos & (c.block - 1)) != c.block - 1) return;
   const int page = p.table[(size_t)b * p.max_blocks + pos / c.block];
   if ((unsigned)page >= (unsigned)c.num_blocks) return;
-  store_new<D>(p, load_new<D>(p, b, kvh), pos, fresh_k, fresh_v);
+  const int i2 = tid & (D / 4 - 1);
+  store_new<D>(load_new<D>(p, b, kvh), reinterpret_cast<const float2*>(p.cos + (size_t)pos * (D / 2))[i2], reinterpret_cast<const float2*>(p.sin + (size_t)pos * (D / 2))[i2], fresh_k, fresh_v);
   __syncthreads();
   const size_t at = ((size_t)b * c.n_kv_heads + kvh) * c.block * D, sc = (size_t)page * c.n_kv_heads + kvh;
   const uint4* k = reinterpret_cast<const uint4*>(c.k_tail + at);
@@ -297,6 +297,10 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
     }
   }
   const NewToken fresh = load_new<D>(p, b, kvh);
+  // The loop's units, in pairs: pair n of this warp is pair warp + W n of the split; a lane looks up the page of one unit of a window of 16 pairs.
+  auto unit_of = [&](int n, int h) { return 2 * (warp + W * n) + h; };
+  const int in_block = 31 - __clz(c.block / 16);  // log2 of the units of a block
+  const int* table = p.table + (size_t)b * p.max_blocks;
   __nv_bfloat16* out = p.out + (size_t)b * p.out_stride + (size_t)head0 * D;
   if (!position_ok(p, pos)) {
     if (split == 0)
@@ -306,12 +310,13 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
   const Split sp = split_of(pos, p);
   if (split >= sp.used) return;
   const bool owns_tail = split == sp.used - 1;
-  const int* table = p.table + (size_t)b * p.max_blocks;
+  // The angles of this lane's dims, for its rows of q and, in the first warp, for k. Behind the loop's loads they would wait for all of those
+  // of the GPU (5 us instead of 1).
+  const float2 cs = reinterpret_cast<const float2*>(p.cos + (size_t)pos * (D / 2))[q_word], sn = reinterpret_cast<const float2*>(p.sin + (size_t)pos * (D / 2))[q_word];
 
-  // ---- the loop's loads: units of the split in pairs, pair n of this warp being pair warp + W n -----------------------------------
+  // ---- the loop's loads -------------------------------------------------------------------------------------------------------------
   const int u0 = split * sp.per, units = max(0, min(sp.units - u0, sp.per));
   const int n_pairs = max(0, ((units + 1) / 2 - warp + W - 1) / W);
-  const int in_block = 31 - __clz(c.block / 16);  // log2 of the units of a block
   const int place = pos & (c.block - 1);
   // the tail's units of 16 positions follow the pairs, the first of them with the last warp
   const int tail_units = owns_tail ? place / 16 + 1 : 0;
@@ -319,8 +324,6 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
   auto tail_first = [&](int n) { return ((W - 1 - warp) + W * (n - n_pairs)) * 16; };
   const size_t tail_at = ((size_t)b * c.n_kv_heads + kvh) * c.block * D;
   bool bad = false;
-  // a window of 16 pairs: each lane looks up the page of one unit, and its scales
-  auto unit_of = [&](int n, int h) { return 2 * (warp + W * n) + h; };
   auto page_of = [&](int n) {  // of window n / 16, for this lane
     const int u = unit_of(n + (lane >> 1), lane & 1);
     if (u >= units) return 0;
@@ -413,7 +416,6 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
   }
 
   // ---- q: rotate, split; the new token ------------------------------------------------------------------------------------------
-  const float2 cs = reinterpret_cast<const float2*>(p.cos + (size_t)pos * (D / 2))[q_word], sn = reinterpret_cast<const float2*>(p.sin + (size_t)pos * (D / 2))[q_word];
 #pragma unroll
   for (int i = 0; i < QI; ++i) {
     const int r = q_row(i);
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
       sm.qc[r] = 128.f * sum * (p.scale * kLog2e / mult);
     }
   }
-  if (owns_tail) store_new<D>(p, fresh, pos, sm.new_k, sm.new_v);
+  if (owns_tail) store_new<D>(fresh, cs, sn, sm.new_k, sm.new_v);  // (q_word is the word that a thread of k has)
   if (tid == 0) sm.bad = 0;
   __syncthreads();
 
@@ -886,12 +888,11 @@ cudaError_t launch(const DecodeAttn8Params& p, cudaStream_t stream) {
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  // Placed before its predecessor has ended, a CTA takes what place that one has left. Where there are fewer CTAs than places some SMs then
-  // have two and others none: 264 of them for 33 ragged sequences take 44.8 us behind themselves, and 35.6 without. Calls of short pieces
-  // and ones that fill the GPU gain what the placing hides (launched one by one: a sequence of 1000 8.8 instead of 10.2 us, 16 of 1087
-  // with 512 CTAs 42.8 instead of 45.0).
-  const bool short_pieces = (long long)p.max_blocks * p.cache.block <= 512LL * p.nsplit, full = pairs * p.nsplit >= 148 * ctas_per_sm(NT, W);
-  cfg.numAttrs = short_pieces || full ? pdl_launch_attr(&attr[0]) : 0;
+  // Placed before its predecessor has ended, a CTA hides its launch (16 sequences of 1087: 34.6 instead of 36.9 us, launched one by one; one of 1000:
+  // 8.1 instead of 10.3). But clusters go where that one leaves room for all their CTAs, and of long pieces some SMs then have two and others
+  // none for long (7 sequences of 65521 in clusters of five, behind themselves: 166 us with, 157 without).
+  const bool short_pieces = (long long)p.max_blocks * p.cache.block <= 512LL * p.nsplit;
+  cfg.numAttrs = short_pieces || !p.cluster ? pdl_launch_attr(&attr[0]) : 0;
   if (p.cluster) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
     attr[cfg.numAttrs].val.clusterDim.x = p.nsplit;
