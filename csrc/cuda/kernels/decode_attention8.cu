@@ -1,22 +1,25 @@
 // Single-token attention over the 8-bit paged cache, fused with rotary embedding, append and the quantisation of a block that fills up.
 //
-// Bound by memory: 2 * head_dim bytes per cached position and KV head. All query heads of a KV head (a tile of eight) go through one CTA,
-// so that a code is read and widened once for them. Per 16 positions a warp multiplies transposed: scores^T = K q^T and then
-// out^T = V^T p^T, with the eight query heads as the N side of m16n8k16. K's rows and V's columns are then the A operand, whose fragments
-// ask of a thread four codes of a row (K) or of a column (V); since the sum over k does not care for its order, a thread takes 16
-// neighbouring bytes of a row and uses them as its k indices of four products (the queries are read in the same order), so that all of K
-// and V goes from global memory into the registers that the products read, 16 bytes a load and whole lines a warp, with no shared memory
-// and no barrier in the loop. (tcgen05 wants its operands in shared memory, widened: a round trip for every byte and 128 rows for at most
-// 16; with eight rows the products take a sixth of the time that the bytes take to arrive.)
+// Bound by memory: 2 * head_dim bytes per cached position and KV head. Measured, of a copy's 6.55 TB/s: 7 sequences of 65521 positions, 64
+// heads on 8, 941 MB: 157 to 168 us, 5.6 to 6.0 TB/s; 16 of 1087, 32 heads, 147 MB: 34.3 us, 4.3 TB/s, of which 2 us pass before the first
+// page is asked for and the launch and the join take as long again; 33 of 0 to 2999, 32 heads on 8, 107 MB: 33 us, by the longest
+// sequence, whose 16 rounds of a warp take 1.4 us each; one of 1000: 8 us, six dependent round trips.
+// All query heads of a KV head (a tile of eight) go through one CTA, so that a code is read and widened once for them. Per 16 positions a
+// warp multiplies transposed: scores^T = K q^T and then out^T = V^T p^T, with the eight query heads as the N side of m16n8k16. K's rows and
+// V's columns are then the A operand, whose fragments ask of a thread four codes of a row (K) or of a column (V); since the sum over k does
+// not care for its order, a thread takes 16 neighbouring bytes of a row and uses them as its k indices of four products (the queries are
+// read in the same order), so that a thread reads 16 bytes at a time what it alone needs, with no barrier in the loop. (tcgen05 wants its
+// operands in shared memory, widened: a round trip for every byte and 128 rows for at most 16; the products keep the tensor pipe busy for
+// 14 % of the time that the bytes take to arrive.)
 //
 // Exactness. Codes widen to f16 without rounding. q is multiplied by a power of two and split into two f16 parts (22 bits), so scores are
 // as exact as in fp32. The page's V scale joins the score, as log2(scale): weights 2^(s + log2 vs - m) multiply the codes in f16, kept
 // within a factor of 2^15 of the running reference, and the sum of the softmax takes them divided by vs, in fp32. The reference m moves
 // only when a score passes it by 2^15, and starts 2^8 below the maximum. The tail (bf16, at most a block) goes through the same products in
-// bf16, q in three parts and the weights in two.
+// bf16, q (the sum of its f16 parts) in three parts and the weights in two.
 //
 // A warp takes two units of 16 positions at a time, so that a fragment of q is read once for both, and has the next two pairs on their way:
-// every thread copies (cp.async) what it will read itself, which needs no barrier. 64 KB of ring let three CTAs of four warps share an SM.
+// every thread copies (cp.async) what it will read itself, which needs no barrier. 16 KB of ring a warp let twelve warps share an SM.
 #include "kv_cache8.cuh"
 
 #include "gemm.h"
@@ -931,6 +934,9 @@ void decode_attention8_split(DecodeAttn8Params& p) {
   const int tile = group > 8 ? 2 : 1, r = 8 * tile;  // query rows of a CTA
   const long long pairs = (long long)p.batch * p.cache.n_kv_heads * ((group + r - 1) / r);
   const long long units = (long long)p.max_blocks * (p.cache.block / 16);  // at most; how long the sequences are only the GPU knows
+  // The CTAs whose number comes nearest to what the GPU holds (us at W 6 / 4 / 3: 512 pairs, 16 sequences of 1087, 41 / 43 / 34; 264 pairs, 33
+  // ragged ones, 33 / 37 / 37; 56 pairs of 65521 positions 157 / 163 / 161; 32 of 1000 8.1 / 8.4 / 8.4). Of equals those that fit at once,
+  // and then the larger.
   double best = 0;
   long long best_waves = 0;
   for (int W : {6, 4, 3}) {

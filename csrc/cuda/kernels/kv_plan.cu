@@ -2,7 +2,8 @@
 //
 // A prefix sum over the requests and then one entry for every token and every new page. The sums are small (a few words a request),
 // so every CTA makes them for itself, in shared memory, and then writes its share of the entries, finding a token's request by binary
-// search; what a plan changes in place (how much is held, the pool's state) is written by one CTA after all have read it: behind a
+// search (1000 requests with 119702 new tokens: 12.5 us, half of it the two launches' sums; one cluster of sixteen for all of it took 13.0.
+// Sixteen requests with 319 tokens: 4.7 us, less than the host's 7.5 for the call); what a plan changes in place (how much is held, the pool's state) is written by one CTA after all have read it: behind a
 // barrier of the one cluster that a plan of ordinary size is, or by a second launch for a large one.
 #include "kv_plan.h"
 

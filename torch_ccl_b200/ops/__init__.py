@@ -1,10 +1,11 @@
-"""Fused collective + compute ops of the `ccl` backend.
+"""Fused collective + compute ops of the `ccl` backend, and the ops beside them that serving and training a language model take: a paged
+8-bit KV cache with its attention (kv_cache.py), log-probabilities over a vocabulary or its shards (logprobs.py).
 
 Every op is registered with the dispatcher as `torch.ops.ccl.<name>` (schema + CUDA kernel + Meta
 kernel for shape inference), so it can be traced with fake tensors, exported and used under
 `torch.compile`; the functions below are thin Python faces that pass the process group by name.
 Each op runs on the CURRENT CUDA stream of the tensor's device (so it can be captured in a CUDA
-graph) through the process group's peer-memory communicator."""
+graph), those with a group through its peer-memory communicator."""
 import torch
 import torch.distributed as dist
 
