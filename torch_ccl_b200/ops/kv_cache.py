@@ -16,6 +16,9 @@ sequence is still filling is held in bf16, in its "tail", and is quantised once,
 scale = max(amax / qmax, 2^-40) with qmax 448 (float8_e4m3fn) or 127 (int8), code = round(x / scale). Attention of position p reads the
 blocks before p // block_size from their pages and the rest from the tail.
 
+A sequence therefore goes on at its next position, or at one that its tail still has (a position of the block that it is filling, whose later
+ones are then written again). It cannot go back to an earlier block: the tail holds another one by then. A page belongs to one request.
+
 Row r of `lengths`, `blocks.table`, the tails and a decode step's qkv belong to the same request; to work on some of them pass slices of
 all (`KVBlocks.rows`, `KVCache8.rows`). All calls run on the current stream of their tensors' device, allocate through torch's allocator
 only and can be captured in a CUDA graph. Two calls that change the same pool, or append to the same rows, must be ordered by the caller.
