@@ -156,3 +156,54 @@ def test_refusals():
         _model("fp8", kv_block=24).prefill(_prompt(1, 8))
     with pytest.raises(AssertionError, match="does not fit"):
         _model("fp8", max_seq=64).prefill(_prompt(1, 65))
+
+
+@pytest.mark.parametrize("fused,captured", [(True, False), (True, True), (False, False)])
+def test_a_sequence_waits_for_a_page_and_goes_on(fused, captured):
+    """Row 1 gets no third page at position 32. It waits there, also past the steps in which its block would have filled up, and once row 0 has ended
+    it goes on with the ids and logits that it has alone in a pool that is large enough."""
+    m, alone = _model("fp8", batch=2, kv_block=16, kv_blocks=5, fused=fused, logprobs=2), _model("fp8", batch=2, kv_block=16, fused=fused)
+    for x in (m, alone):
+        x.prefill(_prompt(2, 31))
+        if captured:
+            x.capture(2)
+    want = []
+    for _ in range(49):
+        ids = alone.decode_step(2)[1].clone()
+        want.append((int(ids), alone.logits[1].clone()))
+    assert int(m.decode_step(2)[1]) == want[0][0]
+    for step in range(1, 22):
+        ids = m.decode_step(2)
+        assert ids[1] == -1 and m.positions.tolist()[1] == 32 and m.last_logprobs.logprob[1] == 0
+        assert (ids[0] == -1) == (step > 16)  # row 0 has pages up to position 47
+    assert m.positions.tolist() == [48, 32] and m.blocks.state.tolist() == [0, 2] and m.waits.tolist() == [True, True]
+    m.finish([0])
+    for ids, logits in want[1:]:
+        got = m.decode_step(2)
+        assert int(got[1]) == ids and torch.equal(m.logits[1], logits) and m.blocks.state.tolist()[1] == 0
+    assert m.positions.tolist()[1] == 80 and m.blocks.held.tolist() == [0, 5]
+
+
+def test_a_serving_loop_hands_back_what_it_got():
+    """Ids go from step to step through the host, -1 among them."""
+    m, alone = _model("int8", batch=2, kv_block=16, kv_blocks=5), _model("int8", batch=2, kv_block=16)
+    got = []
+    for x in (m, alone):
+        x.prefill(_prompt(2, 31))
+        ids, out, mine = x.tokens.cpu().pin_memory(), torch.zeros(2, dtype=torch.int64).pin_memory(), []
+        for step in range(40):
+            if x is m and step == 30:
+                x.finish([0])
+            x.decode_step_host(ids, out)
+            ids.copy_(out)
+            mine.append(int(out[1]))
+        got.append([i for i in mine if i >= 0])
+    assert len(got[0]) == 11 and got[0] == got[1][:11]  # the first step, and those from the 31st on
+
+
+def test_a_sequence_at_the_end_of_its_room_waits():
+    for kv_block in (16, 32):  # of 40 positions: three blocks, and two
+        m = _model("fp8", batch=1, max_seq=40, kv_block=kv_block)
+        m.prefill(_prompt(1, 38))
+        ids = [int(m.decode_step(1)[0]) for _ in range(5)]
+        assert all(i >= 0 for i in ids[:2]) and ids[2:] == [-1] * 3 and m.positions.tolist() == [40]

@@ -146,8 +146,9 @@ class TPLlamaDecoder:
         (7 per layer); kept for A/B measurements. collective="nccl" implies fused=False.
 
         kv_cache: "bf16" (dense, max_seq positions a sequence), or "fp8" / "int8": pages of kv_block positions (16, 32, 64 or 128) with one
-        scale each, kv_blocks of them for all sequences (default: as many as max_batch sequences of max_seq need). A step that the
-        pool has too few pages for leaves `blocks.state[1]` (sequences not served) above zero; such a sequence's results are void.
+        scale each, kv_blocks of them for all sequences (default: as many as max_batch sequences of max_seq need). A sequence that the
+        pool has no page for waits: its id of the step is -1 (with log-probability 0), its token and position stay, and the steps that follow
+        try again, so that it goes on as if nothing had happened once others have ended. `blocks.state[1]` says how many wait.
         logprobs: None, or how many alternatives (0 to 32) `last_logprobs` gives beside the log-probability of every sampled id."""
         self.cfg = cfg
         self.device = torch.device(device if device is not None else f"cuda:{torch.cuda.current_device()}")
@@ -211,6 +212,7 @@ class TPLlamaDecoder:
         self.tokens = torch.zeros(B, device=dev, dtype=torch.int64)
         self.positions = torch.zeros(B, device=dev, dtype=torch.int32)
         self.next_tokens = torch.zeros(B, device=dev, dtype=torch.int64)
+        self.waits = torch.zeros(B, device=dev, dtype=torch.bool)  # sequences that have no page for their position
         self.h = torch.zeros(B, H, **bf)
         self.x = torch.zeros(B, H, **bf)
         self.xn = torch.zeros(B, H, **bf)
@@ -276,9 +278,25 @@ class TPLlamaDecoder:
             _C.decode_attention(qkv, L["k"], L["v"], positions, self.cos, self.sin, attn, self.scratch, self.counters, self.nh, self.nkv, self.nsplit)
 
     def _take_pages(self, B):
-        """Pages for one more position of each of B sequences (none for rows whose position is negative)."""
+        """Pages for one more position of each of B sequences (none for rows whose position is negative). Returns the tokens of the step."""
+        if self.blocks is None:
+            return None
+        kv_plan(self.positions[:B], None, self.blocks.rows(0, B), self.kv_block)
+        room = self.blocks.held[:B] * self.kv_block
+        if self.max_seq % self.kv_block:
+            room.clamp_(max=self.max_seq)
+        torch.ge(self.positions[:B], room, out=self.waits[:B])
+        return self.tokens[:B].clone()
+
+    def _hold_back(self, B, tokens):
+        """After sampling: sequences without a page stay at their token and position. (If they went on, the block that they fill would be lost, and
+        the page that they get for it later would have what its last owner left there.) The place in the tail that this step wrote is
+        written again."""
         if self.blocks is not None:
-            kv_plan(self.positions[:B], None, self.blocks.rows(0, B), self.kv_block)
+            waits = self.waits[:B]
+            torch.where(waits, tokens, self.tokens[:B], out=self.tokens[:B])
+            self.positions[:B].add_(waits, alpha=-1)
+            self.next_tokens[:B].masked_fill_(waits, -1)
 
     def _leave_logprobs(self, B):
         if self.logprobs is not None:
@@ -321,13 +339,14 @@ class TPLlamaDecoder:
         self.comm.embed_norm(tokens, self.embed, self.rank * self.vshard, h, self.layers[0]["attn_norm"], xn, cfg.eps)
         fused_rows = self._fused_rows(B)
         layer = self._layer_fused if fused_rows else self._layer_unfused
-        self._take_pages(B)
+        before = self._take_pages(B)
         for li in range(cfg.n_layers):
             layer(li, B, self.positions[:B])
         self._gemm_t(self.lm_head, xn, self.logits[:B], self.vshard)
         # feeds the sampled ids back into self.tokens and advances the positions: steady state is a pure replay
         # (batches above the fused rows choose among NaNs as torch.max does, like the unfused step)
         self.comm.sample(self.logits[:B], self.next_tokens[:B], tokens, self.positions[:B], nan_first=not fused_rows)
+        self._hold_back(B, before)
         self._leave_logprobs(B)
 
     def _decode_body_unfused(self, B):
@@ -336,7 +355,7 @@ class TPLlamaDecoder:
         self._embed_partial(tokens, x)
         h.zero_()
         self.comm.ar_res_norm(x, h, self.layers[0]["attn_norm"], xn, cfg.eps)
-        self._take_pages(B)
+        before = self._take_pages(B)
         for li in range(cfg.n_layers):
             self._layer_unfused(li, B, self.positions[:B])
         self._gemm_t(self.lm_head, xn, self.logits[:B], self.vshard)
@@ -351,6 +370,7 @@ class TPLlamaDecoder:
             self.next_tokens[:B] = idx
         self.positions[:B] += 1
         self.tokens[:B] = self.next_tokens[:B]  # feed the sampled ids back: steady state is a pure replay
+        self._hold_back(B, before)
         self._leave_logprobs(B)
 
     def capture(self, B):
@@ -381,7 +401,8 @@ class TPLlamaDecoder:
 
     def decode_step(self, B=None):
         """One token for each of the B sequences: reads self.tokens / self.positions, writes
-        self.next_tokens and advances the positions. Device-side only."""
+        self.next_tokens and advances the positions. Device-side only. (8-bit cache: -1 and no advance for a
+        sequence that waits for a page.)"""
         B = B or self.graph_batch or self.max_batch
         if self.graph is not None and self.graph_batch == B:
             self.graph.replay()
@@ -392,9 +413,14 @@ class TPLlamaDecoder:
 
     def decode_step_host(self, tokens_pinned, out_pinned):
         """End-to-end step for a serving loop: token ids come from pinned host memory and the
-        sampled ids are read back to pinned host memory."""
+        sampled ids are read back to pinned host memory. With an 8-bit cache an id of -1, which a sequence that waits for a page has got, stands
+        for the token that it waits with."""
         B = tokens_pinned.numel()
-        self.tokens[:B].copy_(tokens_pinned, non_blocking=True)
+        if self.blocks is None:
+            self.tokens[:B].copy_(tokens_pinned, non_blocking=True)
+        else:
+            given = tokens_pinned.to(self.device, non_blocking=True)
+            torch.where(given < 0, self.tokens[:B], given, out=self.tokens[:B])
         self.decode_step(B)
         out_pinned.copy_(self.next_tokens[:B], non_blocking=True)
         torch.cuda.current_stream(self.device).synchronize()

@@ -18,6 +18,8 @@ blocks before p // block_size from their pages and the rest from the tail.
 
 A sequence therefore goes on at its next position, or at one that its tail still has (a position of the block that it is filling, whose later
 ones are then written again). It cannot go back to an earlier block: the tail holds another one by then. A page belongs to one request.
+A request that a plan did not serve (`blocks.held[r] * block_size` says how many positions it has pages for) has to wait with its position until one
+does: a block that fills up without a page is lost, and a page that is handed out for it later has what its last owner left there.
 
 Row r of `lengths`, `blocks.table`, the tails and a decode step's qkv belong to the same request; to work on some of them pass slices of
 all (`KVBlocks.rows`, `KVCache8.rows`). All calls run on the current stream of their tensors' device, allocate through torch's allocator
