@@ -207,3 +207,19 @@ def test_a_sequence_at_the_end_of_its_room_waits():
         m.prefill(_prompt(1, 38))
         ids = [int(m.decode_step(1)[0]) for _ in range(5)]
         assert all(i >= 0 for i in ids[:2]) and ids[2:] == [-1] * 3 and m.positions.tolist() == [40]
+
+
+def test_a_prompt_that_was_refused_leaves_idle_rows():
+    m, alone = _model("fp8", batch=3, kv_block=16, kv_blocks=7), _model("fp8", batch=3, kv_block=16)
+    with pytest.raises(RuntimeError, match="too few"):
+        m.prefill(_prompt(3, 40))
+    assert m.blocks.state.tolist()[0] == 7 and m.blocks.held.tolist() == [0] * 3 and max(m.positions.tolist()) < 0
+    before = [t.clone() for L in m.layers for t in L["cache"][4:]]
+    for _ in range(3):
+        m.decode_step(3)
+    assert m.blocks.held.tolist() == [0] * 3 and all(torch.equal(a, b) for a, b in zip(before, [t for L in m.layers for t in L["cache"][4:]]))
+    for x in (m, alone):
+        x.prefill(_prompt(2, 40))
+        for _ in range(6):
+            x.decode_step(2)
+    assert torch.equal(m.logits[:2], alone.logits[:2])

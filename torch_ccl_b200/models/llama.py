@@ -436,7 +436,9 @@ class TPLlamaDecoder:
         the communicator's staging arena). After the attention of the last layer only the last position of each
         sequence is wanted: the rest of that layer runs for those rows alone, with the sums over K in the order that
         they have for all rows (no split), so that a prompt's results do not depend on the shortcut.
-        `chunk_seqs` bounds the sequences per pass (default: as many as keep a pass under ~32k rows)."""
+        `chunk_seqs` bounds the sequences per pass (default: as many as keep a pass under ~32k rows). The prompts take rows 0 .. B - 1 of the batch;
+        with an 8-bit cache the pages that those rows held go back to the pool first, and if it has too few for the prompts, the rows are idle
+        (as after `finish`) and a RuntimeError says so."""
         self._prefill(prompt, chunk_seqs, None)
 
     def score(self, prompt, top=0, chunk_seqs=None):
@@ -541,6 +543,7 @@ class TPLlamaDecoder:
         self.positions[:B] = S
         torch.cuda.synchronize(dev)
         if any(int(r) for r in refused):
+            self.finish(range(B))  # what was appended is not whole
             raise RuntimeError(f"prefill: the KV pool of {self.blocks.free.numel()} pages of {self.kv_block} positions has too few for {B} prompts of {S}")
         return TokenLogprobs(*(None if p[0] is None else torch.cat(p) for p in zip(*scored))) if scored else None
 
