@@ -178,7 +178,8 @@ __device__ __forceinline__ void do_cache(const KvAppend8Params& p, int row0, int
       if (ends && row != first && place0 != 0) continue;          // ... which the CTA of the first unit does
       do_unit<D, INT8, IS_K, HEADS>(p, u, kvh0, s_amax, row == row0 && u.n == block, lo, hi);
       if (row == first && place0 != 0 && !ends) {
-        const int last = min(p.starts[u.request + 1], p.rows) - 1;
+        // its last row, or the last that has an angle
+        const int last = min(min(p.starts[u.request + 1], p.rows) - 1, row + (p.table_rows - 1 - p.positions[row]));
         const int tail_row = last - (p.positions[last] & (block - 1));  // where the last block starts
         if (last > row && tail_row >= row + u.n && row_ok(p, tail_row) && p.requests[tail_row] == u.request) {
           const Unit e = unit_at(p, tail_row);

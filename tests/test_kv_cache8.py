@@ -430,6 +430,35 @@ def test_append_skips_what_is_outside():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("before", [0, 5, 16, 19])
+@pytest.mark.parametrize("angles", [24, 33, 40, 47, 48, 49, 63, 64])
+def test_append_up_to_the_end_of_the_rotary_tables(angles, before, dtype):
+    """Rows with an angle are what they are in a prompt that ends there, those without one are left alone, wherever the request and the tables end."""
+    end, block, kv, heads, dim = 64, 16, 3, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(angles + before)
+    qkv = torch.randn(end - before, (heads + 2 * kv) * dim, generator=g, device="cuda").to(BF16)
+    old = torch.randn(2, 1, kv, block, dim, generator=g, device="cuda").to(BF16)
+    cos, sin = tables(end, dim)
+
+    def go(rows, angles):
+        blocks, cache = ops.KVBlocks.empty(1, 5, 9), ops.KVCache8.empty(9, kv, block, dim, 1, dtype)
+        cache.k_tail.copy_(old[0])
+        cache.v_tail.copy_(old[1])
+        admitted([before], [end - before], block, blocks)  # the same pages for both
+        plan = ops.kv_plan(i32([before]), i32([rows]), blocks, block, rows)
+        out = torch.full((rows, (heads + kv) * dim), 7.0, device="cuda", dtype=BF16)
+        ops.kv_append_8bit(qkv[:rows], plan, cache, cos[:angles].contiguous(), sin[:angles].contiguous(), heads, out=out)
+        return out, cache
+
+    n = angles - before
+    out, cache = go(end - before, angles)
+    want, want_cache = go(n, end)
+    assert torch.equal(out[:n], want) and (out[n:] == 7).all()
+    for a, b in zip(cache, want_cache):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # ---- all together --------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,block,dim", [(E4M3, 16, 128), (I8, 32, 64)])
