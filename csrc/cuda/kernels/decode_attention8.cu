@@ -429,8 +429,8 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
 #pragma unroll
     for (int x = LPR / 2; x; x >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
     const int e = (int)(__float_as_uint(most) >> 23);  // biased exponent; 0 for a row of zeros, 255 for an infinity
-    // the largest element at 2^9 .. 2^10, after the factor that half of an e4m3 K's dims get
-    const int up = e == 0 || e == 255 ? 127 : min(254, 127 + (INT8 ? 9 : 1) + 127 - e);
+    // the largest element at 2^9 .. 2^10, after the factor that half of an e4m3 K's dims get (2^8, and finite with it)
+    const int up = e == 0 || e == 255 ? 127 : min(INT8 ? 254 : 246, 127 + (INT8 ? 9 : 1) + 127 - e);
     const float mult = __uint_as_float((uint32_t)up << 23), to_f16 = !INT8 && (q_word & 2) ? mult * kLowE4m3 : mult;
     float sum = 0.f;
 #pragma unroll

@@ -230,6 +230,17 @@ def test_large_and_small_queries():
     assert ((out[3] - best).abs() <= best.abs() * 2.0**-8 + best.abs() * 2.0**-11 + 1e-6).all()
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_queries_down_to_the_smallest(dim, dtype):
+    """Rows whose largest element is anywhere between 2^-100 and the smallest bf16 number: all positions weigh the same."""
+    exponents = list(range(-100, -136, -1))
+    w = World([40 + i for i in range(len(exponents))], 1, 4, 16, dim, dtype)
+    for b, e in enumerate(exponents):
+        w.qkv[b, :4 * dim] *= 2.0**e
+    w.check(attend)
+
+
 def test_nan_and_infinity_stay_where_they_are():
     """A page with a NaN spoils its own sequence and KV head, in whatever way, and no other."""
     w = World([100, 100, 100], 2, 2, 16, 128, E4M3)
