@@ -606,7 +606,8 @@ __global__ void __launch_bounds__(W * 32, ctas_per_sm(NT, W)) decode_attention8_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float rest = INT8 ? ulv - off[a][e & 1] * uks : ulv;
-          s[a][h][e] = (acc[0][a][h][e] + acc[1][a][h][e]) * (f[a][e & 1] * uks) + rest;
+          const float x = (acc[0][a][h][e] + acc[1][a][h][e]) * (f[a][e & 1] * uks) + rest;
+          s[a][h][e] = x + (x - x);  // (what passes fp32 is NaN: -inf would be that or nothing, by what else the warp has)
           if (h == 1 && !there) s[a][h][e] = -INFINITY;
         }
     }

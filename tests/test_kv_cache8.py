@@ -276,6 +276,25 @@ def test_what_is_not_finite_is_not_a_number_in_every_split(at, dtype):
 
 
 @pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("at", [100, 3000, 20000])
+def test_scores_below_fp32_are_not_a_number_either(at, dtype):
+    """Whatever other positions the warp that reads them has: pages of one block, of four and of eight with scores of -2^147."""
+    for pages in (1, 4, 8):
+        w = World([at, 40], 1, 4, 16, 128, dtype)
+        w.cos.fill_(1)
+        w.sin.zero_()
+        w.qkv[0, :4 * 128] = 2.0**70
+        w.qkv[0, 4 * 128:5 * 128] = 0
+        w.cache.k_tail[0] = 0
+        w.cache.k_scale[w.table[0, :at // 16].long()] = 2.0**-80
+        low = w.table[0, :min(pages, at // 16)].long()
+        w.cache.k.view(torch.uint8)[low] = torch.full((), -1.0, device="cuda").to(dtype).view(torch.uint8)
+        w.cache.k_scale[low] = 2.0**70
+        out = attend(w)
+        assert torch.isnan(out[0]).all() and not torch.isnan(out[1]).any()
+
+
+@pytest.mark.parametrize("dtype", [E4M3, I8])
 def test_an_infinity_in_a_block_that_fills_up(dtype):
     """In the tail it is the new token's own; once the block is a page, everything that reads it is NaN."""
     for part in (0, 1):
