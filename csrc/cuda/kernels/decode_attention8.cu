@@ -108,7 +108,7 @@ __device__ __forceinline__ void widen_e4m3(uint32_t w, uint32_t& lo, uint32_t& h
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 // ... 2^-8 of their values, on the integer units: a code's seven lower bits, moved to bit 7, are the f16 whose exponent is read with a bias
-// that is 8 larger, denormals too. (The NaN code has a NaN scale.)
+// that is 8 larger, denormals too. (The NaN code would be 480: a block with a NaN has a NaN scale, which spoils every score of its page.)
 constexpr float kLowE4m3 = 256.f;
 __device__ __forceinline__ void widen_e4m3_low(uint32_t w, uint32_t& lo, uint32_t& hi) {
   const uint32_t x = __byte_perm(w, 0, 0x1100), y = __byte_perm(w, 0, 0x3322);

@@ -307,6 +307,29 @@ def test_an_infinity_in_a_block_that_fills_up(dtype):
         assert torch.isnan(out[0]).all() and not torch.isnan(out[1]).any()
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_a_block_with_a_nan_or_an_infinity_spoils_its_page(value, dtype):
+    """Whoever quantises it gives it a scale that is not finite, and the heads that read it, and no others, are NaN."""
+    for part in (0, 1):
+        w = World([31, 31], 2, 2, 16, 128, dtype)  # a token fills the block
+        w.cache[4 + part][0, 1, 3, 7] = value
+        attend(w)
+        w.at, w.positions = [32, 32], i32([32, 32])
+        out = attend(w).view(2, 4, 128)
+        assert not torch.isfinite(w.cache[2 + part][int(w.table[0, 1]), 1])
+        assert torch.isnan(out[0, 2:]).all() and not torch.isnan(out[0, :2]).any() and not torch.isnan(out[1]).any()
+        blocks, cache = ops.KVBlocks.empty(2, 3, 6), ops.KVCache8.empty(6, 2, 16, 128, 2, dtype)  # a prompt does
+        qkv = torch.randn(64, 8 * 128, generator=w.g, device="cuda").to(BF16)
+        qkv[19, (4 + 2 * part + 1) * 128 + 70] = value  # position 19 of the first request, the second KV head
+        plan = ops.kv_plan(i32([0, 0]), i32([32, 32]), blocks, 16, 64)
+        ops.kv_append_8bit(qkv, plan, cache, w.cos, w.sin, 4)
+        assert [bool(torch.isfinite(cache[2 + part][p, h])) for p in blocks.table[0, :2].tolist() for h in range(2)] == [True, True, True, False]
+        ops.kv_plan(w.positions, None, blocks, 16)
+        out = ops.decode_attention_8bit(w.qkv, w.positions, blocks.table, cache, w.cos, w.sin, 4).view(2, 4, 128)
+        assert torch.isnan(out[0, 2:]).all() and not torch.isnan(out[0, :2]).any() and not torch.isnan(out[1]).any()
+
+
 def test_pages_outside_the_pool():
     """Rows of zeros for a sequence with such a page, in the same split or another, and its token is still appended."""
     at = [100, 100, 3000, 15]

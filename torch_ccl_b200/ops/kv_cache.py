@@ -115,7 +115,9 @@ def decode_attention_8bit(qkv, positions, table, cache, cos, sin, n_heads, out=N
     """One new token per sequence: rotary embedding, append, attention over positions 0 .. positions[b]; returns bf16
     [batch, n_heads * head_dim]. n_heads may be any multiple of the KV heads. A position outside the table or the rotary tables (-1: no
     sequence in this row) gives a row of zeros and appends nothing; so does a row that reads a page number outside the pool, except
-    that its token is appended. A page with an infinity or a NaN, and scores that pass fp32, give NaN for the heads that read them."""
+    that its token is appended. A page with an infinite or NaN scale, which is what a block with an infinity or a NaN is given, and scores that
+    pass fp32, give NaN for the heads that read them. (A NaN among the codes of a page with a finite scale, which nothing here
+    writes, is read as some number.)"""
     if out is None:
         return _ops.decode_attention_8bit.default(qkv, positions, table, *cache, cos, sin, n_heads)
     _ops.decode_attention_8bit_out.default(qkv, positions, table, *cache, cos, sin, n_heads, out)
