@@ -92,7 +92,8 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
 }
 
 // The same in the loop over a row, where m is a whole number of powers of two: x log2 e - m is one multiply-add without an error in m, and sums
-// join exactly. A value that is masked (-inf, or the type's lowest) is raised to where its exponential is still zero but 0 * d is not NaN.
+// join exactly. A value that is masked (-inf, or the type's lowest) is raised to where its exponential beside any other is still zero but 0 * d
+// is not NaN.
 // Rows that this does not hold for (nothing but masked values, infinities, NaN) are found by their sums and done again with Sums.
 struct FastSums {
   float m, s, t;
@@ -105,7 +106,9 @@ __device__ __forceinline__ void rebase(FastSums& a, float m) {
   a.m = m;
 }
 __device__ __forceinline__ void raise_to(FastSums& a, float most) {
-  if (fmaf(most, kLog2e, -a.m) > kLag) rebase(a, rintf(most * kLog2e));
+  // The product rounded up: the nearest number may lie further below a masked value's product than e^x takes, and an infinite sum would send
+  // the whole row through value by value (4095 x 32000 fp32, the first half masked: 199 instead of 82 us).
+  if (fmaf(most, kLog2e, -a.m) > kLag) rebase(a, rintf(__fmul_ru(most, kLog2e)));
 }
 __device__ __forceinline__ void add(FastSums& a, float x) {
   const float d = fmaf(x, kLog2e, -a.m), e = ex2(d);

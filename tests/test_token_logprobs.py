@@ -102,6 +102,23 @@ def test_masks_ties_and_what_is_not_finite(dtype, vocab):
         check(x, t, top)
 
 
+@pytest.mark.parametrize("dtype,mask", [(d, m) for d in (BF16, F32) for m in (-1e4, -1e9, -1e10, -1e20, -1e30, -2.0**100, -1e36, torch.finfo(d).min, -INF)] +
+                         [(F16, m) for m in (-1e4, -65504.0, -INF)])
+@pytest.mark.parametrize("rows,vocab", [(33, 32000), (33, 1000), (2, 128256)])
+def test_masked_ranges_stay_in_the_pass_that_streams(rows, vocab, dtype, mask):
+    """Threads that start on masked values, with any value that masks have. The reference that comes with the results is a whole power of two only
+    if the row went through that pass; one that was done again, value by value, has one of its logits."""
+    x, t = inputs(rows, vocab, dtype, 1)
+    x[:, vocab // 8:] = mask
+    x[:, : vocab // 16] = mask
+    t = t % (vocab // 16) + vocab // 16
+    check(x, t, 0)
+    check(x, t, 5)
+    reference = torch.ops.ccl.token_logprobs(x, t, 0)[2][:, 0].double() * 1.4426950408889634
+    # (a few units, rounded to fp32: 2^-20)
+    assert ((reference - reference.round()).abs() <= 2.0**-19).all()
+
+
 def test_targets_that_are_none():
     x, t = inputs(6, 5000, F32)
     t[1], t[3], t[4] = -1, -100, 5000
