@@ -521,6 +521,7 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   }
 };
 Logprobs token_logprobs_autograd(const Tensor& logits, const Tensor& targets, int64_t top) {
+  TORCH_CHECK(!logits._fw_grad(0).defined(), "token_logprobs: forward-mode derivatives are not implemented");  // (below autograd they would be dropped)
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     auto out = TokenLogprobs::apply(logits, targets, top);
     return {out[0], out[1], out[2], out[3], out[4]};
@@ -576,5 +577,6 @@ TORCH_LIBRARY_IMPL(ccl, Meta, m) {
 
 TORCH_LIBRARY_IMPL(ccl, Autograd, m) {
   m.impl("token_logprobs", &token_logprobs_autograd);
-  m.impl("token_logprobs_backward", torch::autograd::autogradNotImplementedFallback());  // a second derivative is an error, not zero
+  // errors, not zeros: a second derivative, and any of the parts that a group's form is made of
+  for (const char* op : {"token_logprobs_backward", "token_logprobs_shard", "token_logprobs_merge"}) m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

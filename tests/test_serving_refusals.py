@@ -167,6 +167,35 @@ def test_logprobs():
         torch.ops.ccl.token_logprobs_merge(meta(2, 5, 13), t, 4, 1000)
 
 
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_of_logprobs_are_refused(grad):
+    """Of the whole vocabulary's form and of a group's parts; not a derivative of zero."""
+    import torch.autograd.forward_ad as fw
+
+    t = meta(5, dtype=torch.int64)
+    calls = [lambda x: ops.token_logprobs(x, t, top=3).logprob, lambda x: torch.ops.ccl.token_logprobs_shard(x, t, 3, 0, 1000),
+             lambda x: torch.ops.ccl.token_logprobs_merge(x.view(2, 250, 10), meta(250, dtype=torch.int64), 3, 1000)[0]]
+    for call in calls:
+        x = meta(5, 1000).requires_grad_(grad)
+        with fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            call(fw.make_dual(x, meta(5, 1000)))
+        with torch.no_grad(), fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            call(fw.make_dual(x, meta(5, 1000)))
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            torch.func.jvp(call, (meta(5, 1000),), (meta(5, 1000),))
+        call(x)
+
+
+def test_derivatives_of_a_groups_parts_are_refused():
+    t = meta(5, dtype=torch.int64)
+    part = torch.ops.ccl.token_logprobs_shard(meta(5, 500).requires_grad_(True), t, 3, 0, 1000)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        part.sum().backward()
+    lp = torch.ops.ccl.token_logprobs_merge(meta(2, 5, 10).requires_grad_(True), t, 3, 1000)[0]
+    with pytest.raises(RuntimeError, match="not implemented"):
+        lp.sum().backward()
+
+
 def test_cpu_tensors_are_refused():
     b = ops.KVBlocks.empty(4, 8, 64, "cpu")
     with pytest.raises(NotImplementedError):

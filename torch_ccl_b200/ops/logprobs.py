@@ -49,7 +49,7 @@ class _ShardLogprobs(torch.autograd.Function):
 
 def token_logprobs(logits, targets, top=0, group=None):
     """log softmax(logits)[row, targets[row]] and the entropy of every row, with the `top` (0 to 32) best ids and their log-probabilities:
-    a `TokenLogprobs`, differentiable in the logits (bf16, fp16 or fp32 [rows, vocabulary]; rows may be strided).
+    a `TokenLogprobs`, differentiable in the logits (bf16, fp16 or fp32 [rows, vocabulary]; rows may be strided) once and in reverse mode.
 
     targets: int64 [rows]; a negative one stands for "no token" (log-probability 0, no gradient from it), one past the vocabulary gives NaN.
     Equal logits are ordered by id; a NaN counts as larger than everything, as in torch.topk. Sums are in fp32. A gradient may
