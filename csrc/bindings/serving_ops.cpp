@@ -8,6 +8,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 #include <torch/torch.h>
 
@@ -531,6 +533,24 @@ Logprobs token_logprobs_autograd(const Tensor& logits, const Tensor& targets, in
   return op.call(logits, targets, top);
 }
 
+// No derivative goes through the 8-bit cache: one in forward mode is an error, and so is a backward pass that comes to a result. (torch's own kernel for
+// that costs the host a microsecond more a call.)
+void kv_autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  const std::string& name = op.schema().name();
+  torch::autograd::edge_list edges;
+  for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size())) {
+    if (!v.isTensor()) continue;
+    const Tensor& t = v.toTensor();
+    TORCH_CHECK(!t._fw_grad(0).defined(), name, ": forward-mode derivatives are not implemented");
+    if (t.requires_grad() && at::GradMode::is_enabled()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  }
+  TORCH_CHECK(edges.empty() || !op.schema().returns().empty(), name, ": with out there are no derivatives, and an argument requires one");
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+  if (edges.empty()) return;
+  Tensor out = stack->back().toTensor();
+  torch::autograd::set_history(out, std::make_shared<torch::autograd::NotImplemented>(name, std::move(edges)));
+}
+
 }  // namespace
 
 #define CACHE_SCHEMA "Tensor(a!) k, Tensor(b!) v, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor(e!) k_tail, Tensor(f!) v_tail, Tensor cos, Tensor sin, int n_heads"
@@ -579,4 +599,5 @@ TORCH_LIBRARY_IMPL(ccl, Autograd, m) {
   m.impl("token_logprobs", &token_logprobs_autograd);
   // errors, not zeros: a second derivative, and any of the parts that a group's form is made of
   for (const char* op : {"token_logprobs_backward", "token_logprobs_shard", "token_logprobs_merge"}) m.impl(op, torch::autograd::autogradNotImplementedFallback());
+  for (const char* op : {"kv_append_8bit", "kv_append_8bit_out", "decode_attention_8bit", "decode_attention_8bit_out"}) m.impl(op, torch::CppFunction::makeFromBoxedFunction<&kv_autograd>());
 }

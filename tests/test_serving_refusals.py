@@ -196,6 +196,33 @@ def test_derivatives_of_a_groups_parts_are_refused():
         lp.sum().backward()
 
 
+@pytest.mark.parametrize("call,rows", [(append, "rows"), (attend, "qkv")])
+def test_derivatives_through_the_cache_are_refused(call, rows):
+    """In forward mode at the call, in reverse mode when a backward pass comes to the result; without a derivative nothing is in the way."""
+    import torch.autograd.forward_ad as fw
+
+    a = make()
+    x = a[rows]
+    width = 6 * 128 if call is append else 4 * 128
+    out = meta(x.shape[0], width, dtype=BF16)
+    with fw.dual_level():
+        for k in ({}, {"out": out}):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dict(a, **{rows: fw.make_dual(x, meta(*x.shape, dtype=BF16))}), **k)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: call(dict(a, **{rows: x})), (x,), (meta(*x.shape, dtype=BF16),))
+    wants = dict(a, **{rows: x.clone().requires_grad_(True)})
+    result = call(wants)
+    assert result.requires_grad
+    with pytest.raises(RuntimeError, match="not implemented"):
+        (result * 2).sum().backward()
+    with pytest.raises(RuntimeError, match="an argument requires one"):
+        call(wants, out=out)
+    with torch.no_grad():
+        assert call(wants, out=out) is out and not call(wants).requires_grad
+    assert not call(a).requires_grad and call(a, out=out) is out
+
+
 def test_cpu_tensors_are_refused():
     b = ops.KVBlocks.empty(4, 8, 64, "cpu")
     with pytest.raises(NotImplementedError):

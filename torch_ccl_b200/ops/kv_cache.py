@@ -23,7 +23,7 @@ does: a block that fills up without a page is lost, and a page that is handed ou
 
 Row r of `lengths`, `blocks.table`, the tails and a decode step's qkv belong to the same request; to work on some of them pass slices of
 all (`KVBlocks.rows`, `KVCache8.rows`). All calls run on the current stream of their tensors' device, allocate through torch's allocator
-only and can be captured in a CUDA graph. Two calls that change the same pool, or append to the same rows, must be ordered by the caller.
+only and can be captured in a CUDA graph. No gradient goes through them: asking for one is an error. Two calls that change the same pool, or append to the same rows, must be ordered by the caller.
 """
 from typing import NamedTuple
 
