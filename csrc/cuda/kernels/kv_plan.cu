@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(const KvPlanParams p)
       const int r = owner_of(s_base, R, i);
       p.b.table[(size_t)r * p.b.max_blocks + s_held[r] + (i - s_base[r])] = p.b.free_blocks[top - 1 - i];
     }
-    for (int i = first; i < p.room; i += step) {
+    for (unsigned n = first; n < (unsigned)p.room; n += step) {  // (n + step may pass 2^31)
+      const int i = (int)n;
       int r = -1, pos = -1, slot = -1;
       if (i < (int)tokens) {
         r = owner_of(s_start, R, i);

@@ -115,6 +115,19 @@ def test_one_token_each_without_a_list():
         lengths = [n + 1 if n >= 0 else n for n in lengths]
 
 
+def test_a_list_with_room_for_two_billion():
+    """The last entries of a list that is as long as one may be: a step of the loop behind them passes 2^31. (26 GB)"""
+    room = 2**31 - 2
+    blocks, _ = pool(2, 4, 8)
+    plan = ops.kv_plan(i32([0, 3]), i32([20, 30]), blocks, 16, room)
+    assert plan.starts.tolist() == [0, 20, 50] and blocks.state.tolist() == [3, 0]
+    assert plan.positions[:50].tolist() == list(range(20)) + list(range(3, 33))
+    for t in plan[1:]:
+        assert t.shape == (room,)
+        for piece in t[50:].split(1 << 28):
+            assert int(piece.amin()) == int(piece.amax()) == -1
+
+
 def test_what_was_planned_last_comes_back_to_its_place():
     blocks, _ = pool(50, 64, 500)
     before = [t.clone() for t in blocks]
