@@ -179,17 +179,17 @@ __global__ void __launch_bounds__(kThreads) kv_release_kernel(const uint8_t* fin
     ptx::cluster_wait();
   }
   const int step = (int)gridDim.x * kThreads;
-  for (int i = (int)blockIdx.x * kThreads + tid; i < blocks; i += step) {
-    const int r = owner_of(s_base, R, i);
+  for (unsigned n = blockIdx.x * kThreads + tid; n < (unsigned)blocks; n += step) {
+    const int i = (int)n, r = owner_of(s_base, R, i);
     int* entry = b.table + (size_t)r * b.max_blocks + (i - s_base[r]);
-    const int at = top + blocks - 1 - i;
+    const long long at = (long long)top + blocks - 1 - i;  // (counts that make no sense may add up to more than the pool, and to 2^31)
     if (at < b.capacity) b.free_blocks[at] = *entry;
     *entry = -1;
   }
   if (blockIdx.x == 0) {
     for (int r = tid; r < R; r += kThreads)
       if (finished[r]) b.held[r] = 0;
-    if (tid == 0) b.state[0] = min(top + blocks, b.capacity);
+    if (tid == 0) b.state[0] = (int)min((long long)top + blocks, (long long)b.capacity);
   }
 }
 

@@ -160,6 +160,19 @@ def test_words_that_make_no_sense_stay_inside_the_arrays():
     torch.cuda.synchronize()
 
 
+def test_counts_that_add_up_to_two_billion_stay_inside_the_stack():
+    """A release of 16384 requests that claim all of the widest table that they may have, in a pool of a few pages. (9 GB)"""
+    R, width, pages = 16384, 131071, 1000
+    blocks = ops.KVBlocks.empty(R, width, pages)
+    guarded = torch.full((pages + 2000,), 77, dtype=torch.int32, device="cuda")
+    guarded[1000:2000] = blocks.free
+    blocks = blocks._replace(free=guarded[1000:2000])
+    blocks.held.fill_(2**31 - 1)
+    ops.kv_release(torch.ones(R, dtype=torch.bool, device="cuda"), blocks)
+    assert int(blocks.state[0]) == pages and not blocks.held.any()
+    assert (guarded[:1000] == 77).all() and (guarded[2000:] == 77).all()
+
+
 def test_rows_of_a_pool_and_a_graph_on_another_stream():
     blocks, model = pool(12, 16, 100)
     lengths, new = i32([7] * 12), i32([1] * 12)
