@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(WARPS * 32, 48 / WARPS) token_logprobs_kernel(
   __syncthreads();
   if (sm.special) {  // the whole row once more, value by value
     sum = nothing();
-    for (int i = tid; i < p.vocab; i += kThreads) {
+    for (unsigned i = tid; i < (unsigned)p.vocab; i += kThreads) {  // (i + kThreads may pass 2^31)
       const float x = Vec<T>::one(row + i);
       if (!(x - sum.m <= kLag)) rebase(sum, x);
       add(sum, x);

@@ -119,6 +119,16 @@ def test_masked_ranges_stay_in_the_pass_that_streams(rows, vocab, dtype, mask):
     assert ((reference - reference.round()).abs() <= 2.0**-19).all()
 
 
+def test_the_largest_vocabulary_value_by_value():
+    """A row of 2^31 - 1 logits (4 GB) whose maximum is so large that it is done again: a step of that loop from its last element passes 2^31."""
+    vocab = 2**31 - 1
+    x = torch.zeros(1, vocab, dtype=BF16, device="cuda")
+    x[0, vocab - 2] = 2.0**20
+    got = ops.token_logprobs(x, torch.tensor([vocab - 2], device="cuda"), 2)
+    assert got.logprob.item() == 0 and got.entropy.item() == 0
+    assert got.top_ids.tolist() == [[vocab - 2, 0]] and got.top_logprobs.tolist() == [[0.0, -(2.0**20)]]
+
+
 def test_targets_that_are_none():
     x, t = inputs(6, 5000, F32)
     t[1], t[3], t[4] = -1, -100, 5000
