@@ -1,7 +1,7 @@
 // Single-token attention over the 8-bit paged cache, fused with rotary embedding, append and the quantisation of a block that fills up.
 //
 // Bound by memory: 2 * head_dim bytes per cached position and KV head. Measured, of a copy's 6.55 TB/s: 7 sequences of 65521 positions, 64
-// heads on 8, 941 MB: 157 to 168 us, 5.6 to 6.0 TB/s; 16 of 1087, 32 heads, 147 MB: 34.3 us, 4.3 TB/s, of which 2 us pass before the first
+// heads on 8, 941 MB: 154 to 168 us, 5.6 to 6.1 TB/s; 16 of 1087, 32 heads, 147 MB: 34.4 us, 4.3 TB/s, of which 2 us pass before the first
 // page is asked for and the launch and the join take as long again; 33 of 0 to 2999, 32 heads on 8, 107 MB: 33 us, by the longest
 // sequence, whose 16 rounds of a warp take 1.4 us each; one of 1000: 8 us, six dependent round trips.
 // All query heads of a KV head (a tile of eight) go through one CTA, so that a code is read and widened once for them. Per 16 positions a
@@ -14,7 +14,8 @@
 //
 // Exactness. Codes widen to f16 without rounding. q is multiplied by a power of two and split into two f16 parts (22 bits), so scores are
 // as exact as in fp32. The page's V scale joins the score, as log2(scale): weights 2^(s + log2 vs - m) multiply the codes in f16, kept
-// within a factor of 2^15 of the running reference, and the sum of the softmax takes them divided by vs, in fp32. The reference m moves
+// within a factor of 2^15 of the running reference (f16 is what the codes are products with: 2^-11 of each weight, where the result is rounded to bf16,
+// 2^-8; a second part would double V's products), and the sum of the softmax takes them divided by vs, in fp32. The reference m moves
 // only when a score passes it by 2^15, and starts 2^8 below the maximum. The tail (bf16, at most a block) goes through the same products in
 // bf16, q (the sum of its f16 parts) in three parts and the weights in two.
 //
@@ -934,7 +935,9 @@ void decode_attention8_split(DecodeAttn8Params& p) {
   const int group = p.n_heads / p.cache.n_kv_heads;
   const int tile = group > 8 ? 2 : 1, r = 8 * tile;  // query rows of a CTA
   const long long pairs = (long long)p.batch * p.cache.n_kv_heads * ((group + r - 1) / r);
-  const long long units = (long long)p.max_blocks * (p.cache.block / 16);  // at most; how long the sequences are only the GPU knows
+  // At most: how long the sequences are only the GPU knows. A table that is much wider than they are costs (16 of 1087: 34 us in one of 8192 positions,
+  // 72 in one of 32768, 215 in one of 131072).
+  const long long units = (long long)p.max_blocks * (p.cache.block / 16);
   // The CTAs whose number comes nearest to what the GPU holds (us at W 6 / 4 / 3: 512 pairs, 16 sequences of 1087, 41 / 43 / 34; 264 pairs, 33
   // ragged ones, 33 / 37 / 37; 56 pairs of 65521 positions 157 / 163 / 161; 32 of 1000 8.1 / 8.4 / 8.4). Of equals those that fit at once,
   // and then the larger.

@@ -1,7 +1,7 @@
 // Rotary embedding of prompt rows and their quantisation into the 8-bit cache's pages, one pass over the QKV projection.
 //
 // Bound by memory: q, k and v are read once, q and k written back rotated (bf16, for the prompt's own attention), k and v written as one
-// byte each (16 x 1024 rows of 32 + 32 + 32 heads: 167 us, 4.9 TB/s). A CTA takes `block` rows of the projection and a few heads of one kind (q, k or v). For k and v its unit is a cache block:
+// byte each (16 x 1024 rows of 32 + 32 + 32 heads: 166 to 173 us, 4.7 to 4.9 TB/s; int8 180). A CTA takes `block` rows of the projection and a few heads of one kind (q, k or v). For k and v its unit is a cache block:
 // one thread per 16 values (8 dims and the 8 that the rotation pairs them with) of a position, so that a whole block is in the registers
 // of the CTA when its largest magnitude is known, and is read once. Rotary tables are loaded once for all heads of the CTA.
 //
@@ -272,7 +272,7 @@ cudaError_t launch(const KvAppend8Params& p, cudaStream_t stream) {
 template <int D, bool INT8>
 cudaError_t by_size(const KvAppend8Params& p, cudaStream_t s) {
   // Two heads of the cache and four of q a CTA, at 64 registers (us at 16 x 1024 rows of 32 + 32 + 32 heads in blocks of 32: two and two
-  // heads 170, four and four 181, one and one 200; of 16: 163, of 64: 180, of 128: 203).
+  // heads 170, four and four 181, one and one 200; of 16: 162, of 64: 178, of 128: 202; int8 175, 180, 191 and 217).
   const int threads = p.cache.block * (D / 16);
   if (threads <= 256) return launch<D, INT8, 2, 4, 256, 4>(p, s);
   if (threads <= 512) return launch<D, INT8, 2, 4, 512, 2>(p, s);

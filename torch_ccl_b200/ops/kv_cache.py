@@ -23,7 +23,8 @@ does: a block that fills up without a page is lost, and a page that is handed ou
 
 Row r of `lengths`, `blocks.table`, the tails and a decode step's qkv belong to the same request; to work on some of them pass slices of
 all (`KVBlocks.rows`, `KVCache8.rows`). All calls run on the current stream of their tensors' device, allocate through torch's allocator
-only and can be captured in a CUDA graph. No gradient goes through them: asking for one is an error. Two calls that change the same pool, or append to the same rows, must be ordered by the caller.
+only and can be captured in a CUDA graph. No gradient goes through them: asking for one is an error. Two calls
+that change the same pool, or append to the same rows, must be ordered by the caller.
 """
 from typing import NamedTuple
 
@@ -90,9 +91,10 @@ class KVCache8(NamedTuple):
 def kv_plan(lengths, new_tokens, blocks, block_size, max_tokens=0):
     """Gives requests the pages that `new_tokens[r]` more positions after `lengths[r]` need (int32 [requests] each; new_tokens None: one
     more each) and lists the new tokens, up to `max_tokens` of them. A request with a negative length or no new tokens is passed over.
-    What a request already holds counts, so that the same plan made twice takes nothing twice. First come, first served: from the first request that
-    the free pages do not suffice for, none gets any; from the first whose tokens do not fit max_tokens (if that is not 0), none is listed;
-    one that would pass the table's width gets nothing. `blocks.state[1]` says how many requests were not served."""
+    What a request already holds counts, so that the same plan made twice takes nothing twice. First come, first served: from the first
+    request that the free pages do not suffice for, none gets any; from the first whose tokens do not fit max_tokens (if that is not 0), none is listed;
+    one that would pass the table's width gets nothing. `blocks.state[1]` says how many requests were not served. The arrays of a plan share
+    one allocation."""
     return KVPlan(*_ops.kv_plan.default(lengths, new_tokens, *blocks, block_size, max_tokens))
 
 

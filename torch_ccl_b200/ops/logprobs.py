@@ -54,6 +54,7 @@ def token_logprobs(logits, targets, top=0, group=None):
     targets: int64 [rows]; a negative one stands for "no token" (log-probability 0, no gradient from it), one past the vocabulary gives NaN.
     Equal logits are ordered by id; a NaN counts as larger than everything, as in torch.topk. Sums are in fp32. A gradient may
     be captured in a graph if no result of the same logits (where they are a leaf) from the default stream is alive; one that is, is an error.
+    The results of a call share one allocation: what is kept for long, or saved, is best cloned.
 
     group: `logits` are this rank's equal shard of the vocabulary (rank 0 has the first ids); every rank passes the same targets, gets
     the whole vocabulary's results, and the gradient of its own shard. None: `logits` have the whole vocabulary."""
