@@ -25,6 +25,9 @@ __device__ __forceinline__ bool row_ok(const KvAppend8Params& p, int row) {
   return r >= 0 && r < p.n_requests && pos >= 0 && pos < p.table_rows;
 }
 
+// Where the rows of `row`'s request end: behind `row` and inside the projection, whatever starts holds.
+__device__ __forceinline__ int end_of(const KvAppend8Params& p, int request, int row) { return max(min(p.starts[request + 1], p.rows), row + 1); }
+
 struct Unit {
   int row, n;        // its first row and how many
   int place;         // place of the first row in the block
@@ -38,8 +41,7 @@ __device__ __forceinline__ Unit unit_at(const KvAppend8Params& p, int row) {
   u.request = p.requests[row];
   const int pos = p.positions[row];
   u.place = pos & (p.cache.block - 1);
-  u.n = min(min(min(p.starts[u.request + 1], p.rows) - row, p.cache.block - u.place), p.table_rows - pos);
-  u.n = max(u.n, 1);
+  u.n = min(min(end_of(p, u.request, row) - row, p.cache.block - u.place), p.table_rows - pos);
   const int slot = p.slots[row];
   u.page = slot < 0 ? -1 : slot / p.cache.block;
   if (u.page >= p.cache.num_blocks) u.page = -1;
@@ -179,7 +181,7 @@ __device__ __forceinline__ void do_cache(const KvAppend8Params& p, int row0, int
       do_unit<D, INT8, IS_K, HEADS>(p, u, kvh0, s_amax, row == row0 && u.n == block, lo, hi);
       if (row == first && place0 != 0 && !ends) {
         // its last row, or the last that has an angle
-        const int last = min(min(p.starts[u.request + 1], p.rows) - 1, row + (p.table_rows - 1 - p.positions[row]));
+        const int last = min(end_of(p, u.request, row) - 1, row + (p.table_rows - 1 - p.positions[row]));
         const int tail_row = last - (p.positions[last] & (block - 1));  // where the last block starts
         if (last > row && tail_row >= row + u.n && row_ok(p, tail_row) && p.requests[tail_row] == u.request) {
           const Unit e = unit_at(p, tail_row);

@@ -483,6 +483,32 @@ def test_append_skips_what_is_outside():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("end", [-2**31, -2**31 + 1, -6, 0, 1, 2**31 - 1])
+@pytest.mark.parametrize("first", [3, 15])
+def test_append_where_a_request_ends_in_front_of_its_rows(first, end):
+    """Nothing is read or written in front of or behind the rows, and another request's are as they are alone."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    cos, sin = tables(64, 128)
+    qkv = torch.randn(48, 3 * 128, generator=g, device="cuda").to(BF16)
+
+    def go(starts):
+        cache = ops.KVCache8.empty(8, 1, 16, 128, 2)
+        wide = torch.full((148, 2 * 128), 7.0, device="cuda", dtype=BF16)
+        # request 1 has the first 32 rows, request 0 the last 16, so that starts[1] is the end of the one and the beginning of the other
+        plan = ops.KVPlan(i32(starts), i32([1] * 32 + [0] * 16), i32(list(range(32)) + [first + i for i in range(16)]), i32(list(range(32)) + [64 + first + i for i in range(16)]))
+        ops.kv_append_8bit(qkv, plan, cache, cos, sin, 1, out=wide[50:98])
+        assert (wide[:50] == 7).all() and (wide[98:] == 7).all()
+        return wide[50:82], [t.float() for t in cache]
+
+    out, cache = go([32, end, 32])
+    want, want_cache = go([32, 48, 32])
+    assert torch.equal(out, want)
+    for a, b in zip(cache[:4], want_cache[:4]):
+        assert torch.equal(a[:2], b[:2])
+    for a, b in zip(cache[4:], want_cache[4:]):
+        assert torch.equal(a[1], b[1])
+
+
 @pytest.mark.parametrize("dtype", [E4M3, I8])
 @pytest.mark.parametrize("before", [0, 5, 16, 19])
 @pytest.mark.parametrize("angles", [24, 33, 40, 47, 48, 49, 63, 64])
